@@ -201,7 +201,7 @@ def _handles(state):
         pkg = _package()
         state["cache"] = pkg.PagedKVCache(state["k_pages"], state["v_pages"])
         state["batch"] = pkg.PagedBatch(state["table"], state["starts"], state["lens"], max_new_tokens=state["most_new"])
-        state["workspace"] = pkg.make_attention_workspace(state["case"]["heads"], state["cache"])
+        state["workspace"] = pkg.make_attention_workspace(state["cache"])
     return _package(), state["cache"], state["batch"]
 
 
