@@ -319,6 +319,95 @@ int b200_w8a8_linear_blocks128(const int8_t *x_i8, const float *x_block_scales, 
                                int64_t ldr, void *y, int y_dtype, int64_t ldy, int m, int k, int n, int act,
                                int x_block_rows, void *stream);
 
+/* ---- paged key / value cache: append and attention --------------------------------- */
+
+/* What a layer needs between its QKV linear and its out linear.  The reference keeps a ring of dense fp32
+ * keys and values per layer and runs its attention over it (src/world_cuda.cu:303-360 allocate it, :1898-2056
+ * upsert and attend); here keys and values live in pages of 16-bit elements that sequences of any length share.
+ *
+ * Element (page, head, token, i) of K and of V is at page * page_stride + head * head_stride +
+ * token * token_stride + i (elements), so pages may be ordered [head][token] or [token][head].
+ * dtype is B200_DT_F16 or B200_DT_BF16, page_tokens 16, 32, 64, 128 or 256, d_head 64 or 128.  k_pages and v_pages
+ * are 16-byte aligned and every stride is a multiple of 8 elements. */
+typedef struct {
+    void *k_pages, *v_pages;
+    int64_t page_stride, head_stride, token_stride;
+    int dtype, n_pages, page_tokens, n_kv_heads, d_head;
+} b200_w8a8_kv_cache;
+
+/* The sequences of one call, all arrays on the device.  The new tokens of sequence s are rows q_starts[s] to
+ * q_starts[s + 1] of the row buffers; kv_lens[s] counts its keys INCLUDING the new tokens, so new token i of n stands
+ * at position kv_lens[s] - n + i.  page_table[s][p / page_tokens] (rows of max_pages entries) is the page that holds
+ * position p.  Entries behind a sequence's last page, and before the first key that a window lets any new token see,
+ * are never read.  Rows behind q_starts[n_seqs] belong to no sequence and are left as they are.
+ * The arrays are read by the kernels, never by the host, so a captured graph follows what they hold at replay.
+ * max_new_tokens is the caller's bound on the new tokens of one sequence; it chooses the kernel and nothing else: a
+ * wrong bound costs time, not results.
+ * A new token whose position is negative (kv_lens[s] smaller than its new tokens) is not appended, and attends to nothing.
+ * A length beyond max_pages * page_tokens, or a page outside [0, n_pages) where a key is needed, is not accessed: the
+ * call's results for that sequence are undefined, and the next entry point returns 1 once, as for a wait that ran out. */
+typedef struct {
+    const int32_t *page_table; /* [n_seqs, max_pages] */
+    const int32_t *q_starts;   /* [n_seqs + 1] */
+    const int32_t *kv_lens;    /* [n_seqs] */
+    int n_seqs, max_pages;
+    int n_tokens;              /* rows of the row buffers */
+    int max_new_tokens;
+} b200_w8a8_kv_batch;
+
+/* Order of the elements that form a rotation's pair j = 0 .. d/2 - 1: (a, b) -> (a cos - b sin, b cos + a sin).
+ * SPLIT reads elements 2j, 2j + 1 and writes j, j + d/2: what b200_w8a8_linear_qkv_heads and the reference do
+ * (src/world_cuda_ops.cu:1229-1305).  HALVES reads and writes j, j + d/2; PAIRS reads and writes 2j, 2j + 1. */
+#define B200_ROPE_NONE 0
+#define B200_ROPE_SPLIT 1
+#define B200_ROPE_HALVES 2
+#define B200_ROPE_PAIRS 3
+
+/* Keys, values and (nullable) queries of the new tokens: element (row, head, i) of q at row * q_token_stride +
+ * head * q_head_stride + i, likewise k and v, so the three may be slices of one QKV row or head-major arrays.  All have
+ * type x_dtype (fp32, fp16, bf16), 16-byte aligned pointers and strides of a multiple of 16 bytes. */
+typedef struct {
+    const void *q, *k, *v;
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    int x_dtype, n_heads;         /* n_heads: heads of q (0 without q) */
+    void *q_out;                  /* the cache's type; NULL without q */
+    int64_t q_out_token_stride, q_out_head_stride;
+    int norm;                     /* 1: RMSNorm of each head of q and k before the rotation, */
+    float eps;                    /*    x / sqrt(mean(x^2) + eps), */
+    const float *q_weight, *k_weight; /* times these [d_head], nullable */
+    int rope_order;               /* B200_ROPE_* */
+    const float *rope_cos, *rope_sin; /* [rope_rows, d_head / 2], dense */
+    int rope_by_position;         /* 0: row of the tables = row of the token; 1: row = position of the token */
+    int rope_rows;
+} b200_w8a8_kv_new;
+
+/* Norm and rotation of the new queries and keys in fp32, one rounding to the cache's type; keys and values go to their
+ * places in the cache, queries to q_out.  Two tokens of one call must not share a place.  Stands in for the ring upsert
+ * between wm_cuda_qkv_fused_rms_rope_i32_dequant and the attention (src/world_cuda.cu:1898-1960). */
+int b200_w8a8_kv_append(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *batch, const b200_w8a8_kv_new *tokens,
+                        void *stream);
+
+/* out[t, h] = sum_j w_j v_j over the keys j that new token t sees, w = softmax of scale * q[t, h] . k_j; query head h
+ * reads key head h / (n_heads / n_kv_heads).  A token at position p sees
+ *   causal_block = 0:     every key of its sequence;
+ *   causal_block = F > 0: keys up to the end of p's block of F positions, j < (p / F + 1) * F (1: plain causal; the tokens
+ *                         of a frame: every frame sees itself and what came before);
+ *   window = W > 0 (needs causal_block): of those, j >= (p / F + 1) * F - W, the last W up to the end of the block.
+ * A token that sees no key gets zeros.  Keys and values behind a sequence's length may hold anything; what stands within
+ * the length and is hidden from a token counts with weight zero, so a NaN or infinity there spreads as zero times it.
+ * q and out have the cache's type, strides in elements (multiples of 8) and 16-byte aligned pointers; they may not overlap.
+ * Scores, softmax and sums are fp32; weights are rounded to the cache's type for the product with the values.
+ * scale must be positive and finite, n_heads a multiple of the cache's n_kv_heads.
+ * workspace: at least b200_w8a8_paged_attention_workspace_size bytes on the current device, 256-byte aligned, its first
+ * 4096 bytes zero before the first call; every call leaves them zero.  Calls that may overlap on the GPU (graphs replayed
+ * on different streams too) need a workspace each.  Stands in for the reference's attention over its ring
+ * (src/world_cuda.cu:1960-2056). */
+size_t b200_w8a8_paged_attention_workspace_size(int d_head);
+int b200_w8a8_paged_attention(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *batch, const void *q,
+                              int64_t q_token_stride, int64_t q_head_stride, void *out, int64_t out_token_stride,
+                              int64_t out_head_stride, int n_heads, float scale, int causal_block, int window,
+                              void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- the linear stack (host-side driver above the operators) ----------------------- */
 
 /* An opaque object that owns the packed int8 weights of n_layers layers plus activation

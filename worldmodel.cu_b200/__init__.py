@@ -21,6 +21,7 @@ LIB_PATH = HERE / "libb200_w8a8.so"
 
 DT_F32, DT_F16, DT_BF16, DT_S32 = 0, 1, 2, 3
 RQ_PLAIN, RQ_RMS = 1, 2
+ROPE_NONE, ROPE_SPLIT, ROPE_HALVES, ROPE_PAIRS = 0, 1, 2, 3
 ACT_NONE, ACT_SILU, ACT_GELU_TANH = 0, 1, 2
 W_ROW_MAJOR, W_SLAB128 = 0, 1
 
@@ -79,6 +80,10 @@ _PROTOTYPES = {
                                                           c_int64, c_void_p, c_int, c_int, c_float, c_void_p]),
     "b200_w8a8_linear_blocks128": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                            c_int64, c_void_p, c_int, c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p]),
+    "b200_w8a8_kv_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),
+    "b200_w8a8_paged_attention_workspace_size": (c_size_t, [c_int]),
+    "b200_w8a8_paged_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int,
+                                          c_float, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "b200_w8a8_stack_create": (c_void_p, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float]),
     "b200_w8a8_stack_destroy": (None, [c_void_p]),
     "b200_w8a8_stack_set_layer": (c_int, [c_void_p, c_int] + [c_void_p] * 8 + [c_int]),
@@ -438,6 +443,172 @@ def weight_file_info(path, verify=True):
     _check(lib().b200_w8a8_weight_file_info(str(path).encode(), *[ctypes.byref(v) for v in vals], int(verify)),
            "weight_file_info")
     return tuple(v.value for v in vals)
+
+
+# ------------------------------------------------------------------ paged key / value cache
+class _Cache(ctypes.Structure):
+    """b200_w8a8_kv_cache of include/b200_w8a8.h."""
+    _fields_ = [("k_pages", c_void_p), ("v_pages", c_void_p), ("page_stride", c_int64), ("head_stride", c_int64),
+                ("token_stride", c_int64), ("dtype", c_int), ("n_pages", c_int), ("page_tokens", c_int),
+                ("n_kv_heads", c_int), ("d_head", c_int)]
+
+
+class _Batch(ctypes.Structure):
+    """b200_w8a8_kv_batch of include/b200_w8a8.h."""
+    _fields_ = [("page_table", c_void_p), ("q_starts", c_void_p), ("kv_lens", c_void_p), ("n_seqs", c_int),
+                ("max_pages", c_int), ("n_tokens", c_int), ("max_new_tokens", c_int)]
+
+
+class _New(ctypes.Structure):
+    """b200_w8a8_kv_new of include/b200_w8a8.h."""
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("q_token_stride", c_int64), ("q_head_stride", c_int64),
+                ("k_token_stride", c_int64), ("k_head_stride", c_int64), ("v_token_stride", c_int64),
+                ("v_head_stride", c_int64), ("x_dtype", c_int), ("n_heads", c_int), ("q_out", c_void_p),
+                ("q_out_token_stride", c_int64), ("q_out_head_stride", c_int64), ("norm", c_int), ("eps", c_float),
+                ("q_weight", c_void_p), ("k_weight", c_void_p), ("rope_order", c_int), ("rope_cos", c_void_p),
+                ("rope_sin", c_void_p), ("rope_by_position", c_int), ("rope_rows", c_int)]
+
+
+def _require(ok, what):
+    if not ok:
+        raise W8A8Error(what)
+
+
+class PagedKVCache:
+    """Keys and values in pages: two CUDA tensors [pages, kv_heads, page_tokens, d_head] of one 16-bit type and the same
+    strides, last dimension contiguous.  A transposed view of [pages, page_tokens, kv_heads, d_head] memory is fine."""
+
+    def __init__(self, k_pages, v_pages):
+        _require(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.dtype == v_pages.dtype,
+                 "k_pages and v_pages are [pages, kv_heads, page_tokens, d_head] of one shape and type")
+        _require(k_pages.stride() == v_pages.stride() and k_pages.stride(3) == 1,
+                 "k_pages and v_pages have the same strides, the last dimension contiguous")
+        _require(k_pages.is_cuda and k_pages.device == v_pages.device, "the pages are on one CUDA device")
+        self.k_pages, self.v_pages, self.dtype, self.device = k_pages, v_pages, k_pages.dtype, k_pages.device
+        pages, heads, page_tokens, d_head = k_pages.shape
+        self.n_kv_heads, self.d_head = heads, d_head
+        self.struct = _Cache(k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3], _dt(k_pages), pages, page_tokens,
+                             heads, d_head)
+        self.ref = ctypes.addressof(self.struct)
+
+
+class PagedBatch:
+    """The sequences of a call (see b200_w8a8_kv_batch): int32 CUDA tensors page_table [seqs, pages], q_starts [seqs + 1]
+    and kv_lens [seqs], which the kernels read at run time, so they may be updated in place between calls.
+    max_new_tokens: the caller's bound on the new tokens of one sequence (None: the rows of the call)."""
+
+    def __init__(self, page_table, q_starts, kv_lens, max_new_tokens=None):
+        import torch
+        seqs = kv_lens.shape[0]
+        _require(page_table.dim() == 2 and page_table.shape[0] == seqs and q_starts.shape == (seqs + 1,),
+                 "page_table is [seqs, pages], q_starts [seqs + 1], kv_lens [seqs]")
+        for t in (page_table, q_starts, kv_lens):
+            _require(t.dtype == torch.int32 and t.is_contiguous() and t.is_cuda and t.device == kv_lens.device,
+                     "page_table, q_starts and kv_lens are contiguous int32 tensors on one CUDA device")
+        self.tensors, self.device = (page_table, q_starts, kv_lens), kv_lens.device
+        self.max_new_tokens = max_new_tokens
+        self.struct = _Batch(page_table.data_ptr(), q_starts.data_ptr(), kv_lens.data_ptr(), seqs, page_table.shape[1], 0, 0)
+
+    def of(self, n_tokens):
+        """The struct for row buffers of n_tokens rows, a copy for every call."""
+        st = _Batch.from_buffer_copy(self.struct)
+        st.n_tokens = n_tokens
+        st.max_new_tokens = n_tokens if self.max_new_tokens is None else self.max_new_tokens
+        return st
+
+
+def _same_device(device, *tensors):
+    for t in tensors:
+        _require(t is None or t.device == device, "all tensors of a call are on the cache's device")
+
+
+def _heads_strides(t, what, heads=None, d_head=None):
+    _require(t.dim() == 3 and t.stride(2) == 1, f"{what} is [tokens, heads, d_head], the last dimension contiguous")
+    _require((heads is None or t.shape[1] == heads) and (d_head is None or t.shape[2] == d_head),
+             f"{what} has shape {tuple(t.shape)}: heads or d_head differ from the cache's")
+    return t.stride(0), t.stride(1)
+
+
+def _call_on(device, fn):
+    """fn(stream) with `device` current, on its current stream."""
+    import torch
+    if torch.cuda.current_device() == device.index:
+        return fn(torch.cuda.current_stream().cuda_stream)
+    with torch.cuda.device(device):
+        return fn(torch.cuda.current_stream().cuda_stream)
+
+
+def kv_append(cache, batch, k, v, q=None, q_out=None, norm_eps=None, q_weight=None, k_weight=None, rope_cos=None,
+              rope_sin=None, rope_order=None, rope_by_position=False):
+    """Writes the new tokens' keys and values to their places in the cache and, with q, the queries to q_out (returned;
+    allocated when None), with the RMSNorm of each head (norm_eps not None) and the rotation (rope_order not None) of
+    queries and keys on the way.  k, v, q: [tokens, heads, d_head] of one type (fp32, fp16, bf16), any strides."""
+    import torch
+    x = _New()
+    n, d = k.shape[0], cache.d_head
+    x.k_token_stride, x.k_head_stride = _heads_strides(k, "k", cache.n_kv_heads, d)
+    x.v_token_stride, x.v_head_stride = _heads_strides(v, "v", cache.n_kv_heads, d)
+    _require(v.shape[0] == n and v.dtype == k.dtype, "k and v have the same rows and type")
+    _same_device(cache.device, batch, k, v, q, q_out, q_weight, k_weight, rope_cos, rope_sin)
+    x.k, x.v, x.x_dtype = k.data_ptr(), v.data_ptr(), _dt(k)
+    _require(q is not None or q_out is None, "q_out without q")
+    if q is not None:
+        x.q_token_stride, x.q_head_stride = _heads_strides(q, "q", None, d)
+        _require(q.shape[0] == n and q.dtype == k.dtype, "q and k have the same rows and type")
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=cache.dtype, device=q.device)
+        _require(q_out.shape == q.shape and q_out.dtype == cache.dtype, "q_out has q's shape and the cache's type")
+        x.q_out_token_stride, x.q_out_head_stride = _heads_strides(q_out, "q_out")
+        x.q, x.q_out, x.n_heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
+    if norm_eps is not None:
+        x.norm, x.eps = 1, norm_eps
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None:
+            _require(w.dtype == torch.float32 and w.shape == (d,) and w.is_contiguous(), f"{name} is fp32 [d_head]")
+            setattr(x, name, w.data_ptr())
+    if rope_order is not None:
+        x.rope_order = rope_order
+    if x.rope_order:
+        _require(rope_cos is not None and rope_sin is not None, "a rotation needs rope_cos and rope_sin")
+        for t in (rope_cos, rope_sin):
+            _require(t.dtype == torch.float32 and t.dim() == 2 and t.shape[1] == d // 2 and t.is_contiguous()
+                     and t.shape[0] == rope_cos.shape[0], "rope_cos and rope_sin are contiguous fp32 [rows, d_head / 2]")
+        x.rope_cos, x.rope_sin, x.rope_rows = rope_cos.data_ptr(), rope_sin.data_ptr(), rope_cos.shape[0]
+        x.rope_by_position = int(rope_by_position)
+    _check(_call_on(cache.device, lambda st: lib().b200_w8a8_kv_append(cache.ref, ctypes.byref(batch.of(n)), ctypes.byref(x), st)),
+           "kv_append")
+    return q_out
+
+
+def make_attention_workspace(cache):
+    """Zero-filled scratch for paged_attention over caches of this head size on this device.  Every call leaves its
+    counters zero, so one buffer serves all calls that do not overlap on the GPU."""
+    import torch
+    with torch.cuda.device(cache.device):
+        nbytes = lib().b200_w8a8_paged_attention_workspace_size(cache.d_head)
+        return torch.zeros(nbytes, dtype=torch.uint8, device=cache.device)
+
+
+def paged_attention(q, cache, batch, scale=None, causal_block=1, window=0, out=None, workspace=None):
+    """Attention of the new tokens' queries q [tokens, heads, d_head] (the cache's type) over the cache; returns out, like q.
+    causal_block 0: every key; 1: causal; F: causal by blocks of F positions.  window: keys seen, 0 for all.
+    scale: 1 / sqrt(d_head) when None.  workspace: from make_attention_workspace (a fresh one when None)."""
+    import torch
+    qt, qh = _heads_strides(q, "q", None, cache.d_head)
+    _require(q.dtype == cache.dtype, "q has the cache's type")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _require(out.shape == q.shape and out.dtype == q.dtype, "out has q's shape and type")
+    ot, oh = _heads_strides(out, "out")
+    if workspace is None:
+        workspace = make_attention_workspace(cache)
+    _same_device(cache.device, batch, q, out, workspace)
+    if scale is None:
+        scale = cache.d_head ** -0.5
+    _check(_call_on(cache.device, lambda st: lib().b200_w8a8_paged_attention(
+        cache.ref, ctypes.byref(batch.of(q.shape[0])), q.data_ptr(), qt, qh, out.data_ptr(), ot, oh, q.shape[1], scale, causal_block, window,
+        workspace.data_ptr(), workspace.numel() * workspace.element_size(), st)), "paged_attention")
+    return out
 
 
 class _Layer(ctypes.Structure):

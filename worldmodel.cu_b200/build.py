@@ -25,6 +25,8 @@ SOURCES = [
     "gemm_i8_tcgen05.cu",
     "gemm_i8_rowq.cu",
     "gemm_i8_blocks128.cu",
+    "kv_append.cu",
+    "paged_attention.cu",
     "mma_rate.cu",
     "pack_weights.cpp",
     "weight_file.cpp",

@@ -284,4 +284,21 @@ int b200_w8a8_linear_blocks128(const int8_t *x_i8, const float *x_block_scales, 
     return linear_blocks128(a, as_stream(stream));
 }
 
+int b200_w8a8_kv_append(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *batch, const b200_w8a8_kv_new *tokens,
+                        void *stream) {
+    if (status_check_entry()) return 1;
+    return kv_append(cache, batch, tokens, as_stream(stream));
+}
+
+size_t b200_w8a8_paged_attention_workspace_size(int d_head) { return paged_attention_workspace_size(d_head); }
+
+int b200_w8a8_paged_attention(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *batch, const void *q,
+                              int64_t q_token_stride, int64_t q_head_stride, void *out, int64_t out_token_stride,
+                              int64_t out_head_stride, int n_heads, float scale, int causal_block, int window,
+                              void *workspace, size_t workspace_bytes, void *stream) {
+    if (status_check_entry()) return 1;
+    return paged_attention(cache, batch, q, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride, n_heads,
+                           scale, causal_block, window, workspace, workspace_bytes, as_stream(stream));
+}
+
 }  // extern "C"

@@ -18,6 +18,8 @@ enum KernelStatus : int {
     KS_TIMEOUT_TMEM_EMPTY = 103,  // MMA issuer waited too long for a drained accumulator
     KS_TIMEOUT_TMEM_FULL = 104,   // epilogue waited too long for a finished accumulator
     KS_TIMEOUT_ROW_EXCHANGE = 105,  // epilogue waited too long for the row statistics of the other CTAs of its cluster
+    KS_TIMEOUT_SOFTMAX = 106,     // attention's MMA issuer waited too long for weights, or its softmax warps for scores
+    KS_BAD_PAGE = 201,            // a length or page index led outside the cache; the access was left out
 };
 
 constexpr unsigned long long kDefaultWaitLimitNs = 2000000000ull;  // 2 s per wait, then give up

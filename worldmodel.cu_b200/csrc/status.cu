@@ -32,6 +32,7 @@ const char *status_text(int code) {
         case KS_TIMEOUT_TMEM_EMPTY: return "the MMA issuer waited too long for a drained accumulator";
         case KS_TIMEOUT_TMEM_FULL: return "the epilogue waited too long for a finished accumulator";
         case KS_TIMEOUT_ROW_EXCHANGE: return "the epilogue waited too long for the row statistics of its cluster";
+        case KS_TIMEOUT_SOFTMAX: return "the attention's scores or weights were waited for too long";
         default: return "unknown status";
     }
 }
@@ -87,6 +88,9 @@ int status_check_entry() {
     cudaDeviceSynchronize();
     *h = 0;
     gemm_reset_static_tickets();
+    if (code == KS_BAD_PAGE)
+        return fail("an earlier append or attention met a sequence length or page index outside its cache (status %d); "
+                    "nothing was accessed there and the results of that sequence are undefined", code);
     return fail("an earlier kernel gave up a bounded wait (status %d: %s); the outputs of that launch are incomplete, "
                 "and a split-K workspace it used must be zeroed again before reuse",
                 code, status_text(code));

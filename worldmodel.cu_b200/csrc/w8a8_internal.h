@@ -202,6 +202,14 @@ unsigned long long *gemm_trace_buffer();
 void gemm_force_plan(int bn, int splits, int mode);
 int gemm_forced_tile_width();  // 0 unless a test forced one
 
+// ---- kv_append.cu, paged_attention.cu: the paged key / value cache
+int kv_append(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *batch, const b200_w8a8_kv_new *tokens,
+              cudaStream_t stream);
+size_t paged_attention_workspace_size(int d_head);
+int paged_attention(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *batch, const void *q, long long q_ts,
+                    long long q_hs, void *out, long long o_ts, long long o_hs, int n_heads, float scale, int causal_block,
+                    int window, void *workspace, size_t workspace_bytes, cudaStream_t stream);
+
 // ---- mma_rate.cu
 int mma_issue_rate(int slabs_per_cta, double *tera_ops_per_s);
 
