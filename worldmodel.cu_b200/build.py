@@ -27,6 +27,7 @@ SOURCES = [
     "gemm_i8_blocks128.cu",
     "kv_append.cu",
     "paged_attention.cu",
+    "paged_attention_chunk.cu",
     "mma_rate.cu",
     "pack_weights.cpp",
     "weight_file.cpp",

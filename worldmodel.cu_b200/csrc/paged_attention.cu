@@ -354,9 +354,9 @@ int current_device_sms(int &dev) {
 
 size_t paged_attention_workspace_size(int d_head) {
     int dev;
-    const int sms = std::min(current_device_sms(dev), kMaxCtas / 2);
+    const int sms = std::min(current_device_sms(dev), kMaxSms);
     const size_t rows = 4ull * sms * kRowTile * (d_head + 2) * sizeof(float);
-    return kTicketBytes + rows;
+    return kTicketBytes + std::max(rows, attention_chunk_partial_bytes(d_head, sms));
 }
 
 int paged_attention(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *batch, const void *q, long long q_ts,
@@ -389,9 +389,13 @@ int paged_attention(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *b
     a.partials = reinterpret_cast<float *>(reinterpret_cast<char *>(workspace) + kTicketBytes);
     a.min_tiles = 4;
     int dev;
-    const int sms = std::min(current_device_sms(dev), kMaxCtas / 2);
+    const int sms = std::min(current_device_sms(dev), kMaxSms);
     AttnDeviceInfo &di = attn_device_info(dev);
     const bool bf = cache->dtype == B200_DT_BF16;
+    if ((long long)batch->max_new_tokens * a.group > kRowTile) {
+        a.min_tiles = 2;
+        return launch_attention_chunk(cache, a, sms, dev, stream);
+    }
     if (cache->d_head == 64)
         return bf ? launch_rows<__nv_bfloat16, 64>(a, sms, di.attr_set[0][1], stream)
                   : launch_rows<__half, 64>(a, sms, di.attr_set[0][0], stream);

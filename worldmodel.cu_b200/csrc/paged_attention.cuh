@@ -12,10 +12,6 @@
 #include "paged_kv.cuh"
 
 namespace b200 {
-namespace {
-
-constexpr int kTicketBytes = 4096;  // one ticket per CTA, at the start of the workspace
-constexpr int kMaxCtas = kTicketBytes / 4;
 
 struct AttnParams {
     KvView c;
@@ -30,6 +26,15 @@ struct AttnParams {
     int *tickets;
     float *partials;
 };
+
+// ---- paged_attention_chunk.cu
+size_t attention_chunk_partial_bytes(int d_head, int sms);
+int launch_attention_chunk(const b200_w8a8_kv_cache *cache, const AttnParams &a, int sms, int dev, cudaStream_t stream);
+
+namespace {
+
+constexpr int kTicketBytes = 16384;           // counters at the start of the workspace: one per warp that joins
+constexpr int kMaxSms = kTicketBytes / 4 / 8;  // eight such warps per SM
 
 // First key and one past the last key that the token at position p (< keys) sees; empty where p is negative.
 __device__ __forceinline__ void visible_keys(const AttnParams &a, int p, int keys, int &lo, int &hi) {

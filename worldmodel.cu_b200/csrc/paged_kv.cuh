@@ -8,7 +8,6 @@
 #include "w8a8_internal.h"
 
 namespace b200 {
-namespace {
 
 struct KvView {
     void *k, *v;
@@ -18,6 +17,8 @@ struct KvView {
     int n_seqs, max_pages, n_tokens;
     int *status;
 };
+
+namespace {
 
 __device__ __forceinline__ void report_bad_page(const KvView &c) {
     if (c.status && *(volatile int *)c.status == 0) {
