@@ -19,6 +19,7 @@ constexpr int kRowsThreads = 128;
 constexpr int kRowTile = 16;  // rows of one matrix instruction
 constexpr int kStepKeys = 16;
 constexpr int kRowsKeyTile = kStepKeys * (kRowsThreads / 32);  // keys per KV tile of the plan
+constexpr int kRowsExtra = 2;
 
 template <int D>
 struct RowsCfg {
@@ -74,10 +75,10 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attention_rows_kernel(const A
     const int g = lane >> 2, t = lane & 3;
     pdl_trigger();
     pdl_wait();
-    long long total, x0, x1;
-    int runs;
+    long long x0, x1;
+    RunMap map;
     Item it;
-    if (!plan_run<kRowTile, kRowsKeyTile, kRowsThreads>(a, plan, total, runs, x0, x1, it)) return;
+    if (!plan_run<kRowTile, kRowsKeyTile, kRowsExtra, kRowsThreads>(a, plan, map, x0, x1, it)) return;
 
     uint8_t *ring = smem + warp * C::kStages * C::kStepBytes;
     const uint32_t ring_addr = smem_u32(ring);
@@ -85,8 +86,9 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attention_rows_kernel(const A
     const T *kb = reinterpret_cast<const T *>(a.c.k), *vb = reinterpret_cast<const T *>(a.c.v);
 
     for (long long x = x0; x < x1;) {
-        const long long end = it.begin + (it.kt1 - it.kt0);
-        const int kt0 = it.kt0 + (int)(x - it.begin), kt1 = it.kt0 + (int)(min(x1, end) - it.begin);
+        int kt0, kt1;
+        const long long upto = run_part<kRowsExtra>(it, x, x1, kt0, kt1);
+        if (kt0 == kt1) break;  // the run ends within the item's EXTRA part: its tiles are the next CTA's
         const int r0 = it.rt * kRowTile, rows = min(kRowTile, it.rows - r0);
 
         // queries: A fragments of the 16 rows
@@ -96,7 +98,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attention_rows_kernel(const A
         for (int j = 0; j < 2; ++j) {
             const int r = r0 + g + 8 * j;
             const bool live = r < it.rows;
-            const int tok = live ? r / a.group : 0, head = live ? it.h * a.group + r % a.group : 0;
+            const int tok = live ? a.by_group.div(r) : 0, head = live ? it.h * a.group + r - tok * a.group : 0;
             lo[j] = hi[j] = 0;
             if (live) visible_keys(a, it.seq.keys - it.seq.n + tok, it.seq.keys, lo[j], hi[j]);
             const T *src = reinterpret_cast<const T *>(a.q) + (long long)(it.seq.q0 + tok) * a.q_ts + head * a.q_hs + 2 * t;
@@ -238,7 +240,8 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attention_rows_kernel(const A
                     make_float2(o[n][2 * r], o[n][2 * r + 1]);
         __syncthreads();
 
-        const int first = run_of(it.begin, total, runs), final = run_of(end - 1, total, runs);
+        const long long begin = it.begin + kRowsExtra;
+        const int first = map.run_of(begin), final = map.run_of(begin + (it.kt1 - it.kt0) - 1);
         const bool whole = first == final;
         float *part = a.partials + (long long)(2 * blockIdx.x + ((int)blockIdx.x == first ? 1 : 0)) * C::kPartialFloats;
         for (int i = threadIdx.x; i < rows * (D / 2); i += kRowsThreads) {
@@ -260,8 +263,9 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attention_rows_kernel(const A
             if (whole) {
                 const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
                 const int rr = r0 + r;
-                T *dst = reinterpret_cast<T *>(a.out) + (long long)(it.seq.q0 + rr / a.group) * a.o_ts +
-                         (long long)(it.h * a.group + rr % a.group) * a.o_hs + col;
+                const int tok = a.by_group.div(rr);
+                T *dst = reinterpret_cast<T *>(a.out) + (long long)(it.seq.q0 + tok) * a.o_ts +
+                         (long long)(it.h * a.group + rr - tok * a.group) * a.o_hs + col;
                 *reinterpret_cast<uint32_t *>(dst) = Half2Of<T>::pack(v.x * inv, v.y * inv);
             } else {
                 *reinterpret_cast<float2 *>(part + r * D + col) = v;
@@ -301,15 +305,16 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attention_rows_kernel(const A
                     }
                     const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
                     const int rr = r0 + r;
-                    T *dst = reinterpret_cast<T *>(a.out) + (long long)(it.seq.q0 + rr / a.group) * a.o_ts +
-                             (long long)(it.h * a.group + rr % a.group) * a.o_hs + col;
+                    const int tok = a.by_group.div(rr);
+                    T *dst = reinterpret_cast<T *>(a.out) + (long long)(it.seq.q0 + tok) * a.o_ts +
+                             (long long)(it.h * a.group + rr - tok * a.group) * a.o_hs + col;
                     *reinterpret_cast<uint32_t *>(dst) = Half2Of<T>::pack(v.x * inv, v.y * inv);
                 }
             }
         }
         __syncthreads();  // the ring and the warp statistics are free again
-        x = min(x1, end);
-        if (x < x1) next_item<kRowTile, kRowsKeyTile>(a, it);
+        x = upto;
+        if (x < x1) next_item<kRowTile, kRowsKeyTile, kRowsExtra>(a, it);
     }
 }
 
@@ -382,6 +387,9 @@ int paged_attention(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *b
     a.q = q; a.q_ts = q_ts; a.q_hs = q_hs;
     a.out = out; a.o_ts = o_ts; a.o_hs = o_hs;
     a.group = n_heads / cache->n_kv_heads;
+    a.by_group.set((unsigned)a.group);
+    a.by_block.set((unsigned)std::max(causal_block, 1));
+    a.by_heads.set((unsigned)cache->n_kv_heads);
     a.scale_log2 = scale * 1.4426950408889634f;
     a.block = causal_block;
     a.window = window;

@@ -18,10 +18,11 @@ namespace b200 {
 namespace {
 
 constexpr int kChunkThreads = 384;  // three warpgroups; warps 10 and 11 only fill the third
-// registers a thread: 384 x 168 at launch = 64512 >= 256 x 208 + 128 x 80 = 63488
-constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
+// registers a thread: 384 x 168 at launch = 64512 = 256 x 224 + 128 x 56
+constexpr int kSoftmaxRegs = 224, kOtherRegs = 56;
 constexpr int kChunkRows = 256;   // two row tiles
 constexpr int kKeyTile = 128;
+constexpr int kChunkExtra = 3;
 constexpr int kSlabBytes = 128 * 128;  // 128 rows of 64 16-bit elements, 128-byte swizzle
 constexpr float kLazyRescale = 8.0f;   // log2 of how far a weight may exceed one
 
@@ -44,19 +45,44 @@ __device__ __forceinline__ uint64_t smem_desc_mn128(uint32_t addr) {
     d |= (uint64_t)2 << 61;
     return d;
 }
-__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// True in one thread of a converged warp.  Unlike `lane == 0` the compiler knows that a branch on it holds a single thread, and
+// feeds the operands of tcgen05 instructions to the uniform registers directly.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(one));
+    return one != 0;
+}
+// Four products over 16 elements of K each: 32 bytes of a K-major row, or 8 columns of weights and 16 rows of values.  One block of assembly with its own arithmetic: left to the compiler, the operands of all unrolled products are
+// kept in registers that the issuing warp does not have.
+__device__ __forceinline__ void umma_f16_ss4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, t;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+        "add.s64 a, %1, 2;\n\tadd.s64 b, %2, 2;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t"
+        "add.s64 a, %1, 4;\n\tadd.s64 b, %2, 4;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t"
+        "add.s64 a, %1, 6;\n\tadd.s64 b, %2, 6;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t}" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
-__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void umma_f16_ts4(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "{\n\t.reg .pred p, t;\n\t.reg .b32 a;\n\t.reg .b64 b;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "add.u32 a, %1, 8;\n\tadd.s64 b, %2, 128;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+        "add.u32 a, %1, 16;\n\tadd.s64 b, %2, 256;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+        "add.u32 a, %1, 24;\n\tadd.s64 b, %2, 384;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t}" ::"r"(d),
         "r"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
@@ -68,6 +94,15 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r
         "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void *map, uint64_t *bar, int c0, int c1, int c2, int c3) {
     asm volatile(
@@ -75,6 +110,59 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void *map, uint6
         "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
         "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
         : "memory");
+}
+
+// two fp32 values per instruction
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair2(uint64_t v, float &a, float &b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 2^x for x in [-inf, 2^22) on the multiply-add pipe: x = n + f, n the nearest integer, |f| <= 1/2; 2^f by the polynomial of
+// least relative error over that interval (degree 3: 7.5e-5, for weights rounded to bf16 by up to 2^-9; degree 4: 2.6e-6,
+// for fp16's 2^-12), n added to the exponent.  Results below 2^-126 become about 2^-126.
+template <int DEGREE>
+__device__ __forceinline__ void poly_ex2(uint64_t x, float &e0, float &e1) {
+    float a, b;
+    unpair2(x, a, b);
+    x = pair2(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+    const float magic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer in the low bits
+    const uint64_t t = add2(x, pair2(magic, magic));
+    const uint64_t f = fma2(add2(t, pair2(-magic, -magic)), pair2(-1.0f, -1.0f), x);
+    uint64_t p;
+    if (DEGREE == 3) {
+        p = fma2(pair2(0.05517132207751274f, 0.05517132207751274f), f, pair2(0.2426113337278366f, 0.2426113337278366f));
+        p = fma2(p, f, pair2(0.6932610869407654f, 0.6932610869407654f));
+        p = fma2(p, f, pair2(0.9999280571937561f, 0.9999280571937561f));
+    } else {
+        p = fma2(pair2(0.00957053154706955f, 0.00957053154706955f), f, pair2(0.05591866374015808f, 0.05591866374015808f));
+        p = fma2(p, f, pair2(0.24024735391139984f, 0.24024735391139984f));
+        p = fma2(p, f, pair2(0.6931216716766357f, 0.6931216716766357f));
+        p = fma2(p, f, pair2(0.9999992847442627f, 0.9999992847442627f));
+    }
+    float p0, p1, t0, t1;
+    unpair2(p, p0, p1);
+    unpair2(t, t0, t1);
+    e0 = __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23));
+    e1 = __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 
 template <typename T>
@@ -90,6 +178,50 @@ template <typename T>
 __host__ __device__ constexpr uint32_t idesc_f16(int n, uint32_t b_mn_major) {
     return (1u << 4) | (IsBf16<T>::value << 7) | (IsBf16<T>::value << 10) | (b_mn_major << 16) | ((uint32_t)(n >> 3) << 17) |
            ((uint32_t)(128 >> 4) << 24);
+}
+
+template <int N>
+struct Int {
+    static constexpr int value = N;
+};
+// Of every 8 pairs of weights, how many the multiply-add pipe computes.
+template <int D>
+constexpr int kPolyPairs = D == 128 ? 2 : 4;
+
+// Waits and commits by shared-memory address: what stands between two products of the issuing thread is kept short.
+__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, const WaitCtx &w, int code) {
+    if (try_wait(bar, parity)) return true;
+    const unsigned long long t0 = global_timer_ns();
+    uint32_t spins = 0;
+    while (!try_wait(bar, parity)) {
+        if (((++spins) & 0x3Fu) == 0) {
+            if (*w.abort_flag) return false;
+            if (global_timer_ns() - t0 > w.limit_ns) {
+                *w.abort_flag = 1;
+                if (w.status && *(volatile int *)w.status == 0) *(volatile int *)w.status = code;
+                __threadfence_system();
+                return false;
+            }
+        }
+    }
+    return true;
+}
+__device__ __forceinline__ void commit_to(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void arrive_on(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 struct ChunkExtra {
@@ -108,28 +240,23 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     __shared__ Item items[10];  // every warp's own place in the plan, kept out of the loops' registers
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *ring = smem + 2 * C::kTileBytes;
-    uint64_t *kv_full = reinterpret_cast<uint64_t *>(ring + C::kStages * C::kTileBytes);
-    uint64_t *kv_empty = kv_full + C::kStages;
-    uint64_t *q_ready = kv_empty + C::kStages;  // [2] the row tile's queries are in shared memory
-    uint64_t *s_full = q_ready + 2;             // [2] scores are in tensor memory
-    uint64_t *p_ready = s_full + 2;             // [2] weights are in tensor memory, O is rescaled
-    uint64_t *o_full = p_ready + 2;             // [2] the last product of a run has landed
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(o_full + 2);
+    // barriers: [stage] pages have landed; [stage] their products are done; [row tile] its queries are in shared memory; its
+    // scores are in tensor memory; [row tile][half] half of its weights are there and O is rescaled; [row tile] the last product
+    // of a run has landed
+    uint64_t *bars = reinterpret_cast<uint64_t *>(ring + C::kStages * C::kTileBytes);
+    const uint32_t kv_full = smem_u32(bars), kv_empty = kv_full + 8 * C::kStages, q_ready = kv_empty + 8 * C::kStages;
+    const uint32_t s_full = q_ready + 16, p_ready = s_full + 16, o_full = p_ready + 32;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * C::kStages + 10);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const WaitCtx wctx{abort_flag, a.c.status, ex.wait_limit_ns};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     pdl_trigger();
     if (threadIdx.x == 0) {
-        for (int s = 0; s < C::kStages; ++s) {
-            mbar_init(&kv_full[s], 1);
-            mbar_init(&kv_empty[s], 1);
-        }
-        for (int x = 0; x < 2; ++x) {
-            mbar_init(&q_ready[x], 4);
-            mbar_init(&s_full[x], 1);
-            mbar_init(&p_ready[x], 4);
-            mbar_init(&o_full[x], 1);
+        // four arrivals, one per softmax warp, where such a warp signals; one everywhere else
+        for (int i = 0; i < 2 * C::kStages + 10; ++i) {
+            const int j = i - 2 * C::kStages;
+            mbar_init(bars + i, j == 0 || j == 1 || (j >= 4 && j < 8) ? 4 : 1);
         }
         *abort_flag = 0;
         fence_mbar_init();
@@ -137,11 +264,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         tma_prefetch_desc(&tm_v);
     }
     pdl_wait();
-    long long total, x0, x1;
-    int runs;
+    long long x0, x1;
+    RunMap map;
     {
         Item first;
-        if (!plan_run<kChunkRows, kKeyTile, kChunkThreads>(a, plan, total, runs, x0, x1, first)) return;
+        if (!plan_run<kChunkRows, kKeyTile, kChunkExtra, kChunkThreads>(a, plan, map, x0, x1, first)) return;
         if (lane == 0 && warp < 10) items[warp] = first;
     }
     Item &it = items[min(warp, 9)];
@@ -164,8 +291,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             bool ok = true, drop = ex.debug_drop_load != 0;
             const int boxes = kKeyTile / ex.page_box;  // along the keys of a tile
             for (long long x = x0; ok && x < x1;) {
-                const long long end = it.begin + (it.kt1 - it.kt0);
-                const int kt0 = it.kt0 + (int)(x - it.begin), kt1 = it.kt0 + (int)(min(x1, end) - it.begin);
+                int kt0, kt1;
+                const long long upto = run_part<kChunkExtra>(it, x, x1, kt0, kt1);
+                if (kt0 == kt1) break;  // the run ends within the item's EXTRA part: its tiles are the next CTA's
                 const int lo = it.lo, hi = it.hi, kv_head = it.h;
                 const int *table = a.c.page_table + (long long)it.s * a.c.max_pages;
                 for (int kt = kt0; ok && kt < kt1; ++kt) {
@@ -184,115 +312,97 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     const unsigned mask = __ballot_sync(0xffffffffu, live);
                     const uint32_t bytes = (uint32_t)__popc(mask) * (uint32_t)ex.page_box * (D * 2);
                     for (int kv = 0; kv < 2; ++kv) {
-                        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&kv_empty[s], ph ^ 1u, wctx, KS_TIMEOUT_SMEM_EMPTY));
+                        ok = __all_sync(0xffffffffu, wait_bounded(kv_empty + 8 * s, ph ^ 1u, wctx, KS_TIMEOUT_SMEM_EMPTY));
                         if (!ok) break;
-                        if (lane == 0) mbar_arrive_expect_tx(&kv_full[s], bytes);
+                        if (lane == 0) mbar_arrive_expect_tx(bars + s, bytes);
                         __syncwarp();
                         if (live && !drop) {
                             const uint32_t dst = smem_u32(ring + s * C::kTileBytes) + (uint32_t)(lane * ex.page_box * 128);
 #pragma unroll
                             for (int d = 0; d < D / 64; ++d)
-                                tma_load_4d(dst + d * kSlabBytes, kv ? &tm_v : &tm_k, &kv_full[s], d * 64, token, kv_head, page);
+                                tma_load_4d(dst + d * kSlabBytes, kv ? &tm_v : &tm_k, bars + s, d * 64, token, kv_head, page);
                         }
                         drop = false;
                         if (++s == C::kStages) { s = 0; ph ^= 1u; }
                     }
                 }
-                x = min(x1, end);
+                x = upto;
                 if (x < x1) {
                     __syncwarp();
-                    if (lane == 0) next_item<kChunkRows, kKeyTile>(a, it);
+                    if (lane == 0) next_item<kChunkRows, kKeyTile, kChunkExtra>(a, it);
                     __syncwarp();
                 }
             }
         } else if (warp == 9) {
-            // ---- products
-            constexpr uint32_t idesc_s = idesc_f16<T>(kKeyTile, 0), idesc_o = idesc_f16<T>(D, 1);
-            int s = 0;
-            uint32_t ph = 0, q_ph = 0, p_ph = 0;  // bit x: parity of the row tile's barrier
-            bool ok = true;
-            auto wait = [&](uint64_t *bar, uint32_t parity, int code) {
-                ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, wctx, code));
-                return ok;
-            };
-            auto scores = [&](int x, int stage) {  // S_x = Q_x K^T, then s_full[x]
-                if (lane == 0) {
-                    const uint64_t qd = umma_smem_desc_k128(smem_u32(smem + x * C::kTileBytes));
-                    const uint64_t kd = umma_smem_desc_k128(smem_u32(ring + stage * C::kTileBytes));
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const uint64_t off = (uint64_t)(((k / 4) * kSlabBytes + (k % 4) * 32) >> 4);
-                        umma_f16_ss(tmem + x * kKeyTile, qd + off, kd + off, idesc_s, k != 0);
-                    }
-                    umma_commit(&s_full[x]);
-                }
-                __syncwarp();
-            };
-            for (long long x = x0; ok && x < x1;) {
-                const long long end = it.begin + (it.kt1 - it.kt0);
-                const int kt0 = it.kt0 + (int)(x - it.begin), kt1 = it.kt0 + (int)(min(x1, end) - it.begin);
-                const int lo = it.lo, hi = it.hi;
-                const int tiles = it.rows - it.rt * kChunkRows > 128 ? 2 : 1;
-                for (int kt = kt0 - 1; ok && kt < kt1; ++kt) {
-                    // V of tile kt and K of tile kt + 1 are the next two stages of the ring
-                    const int vs = s;
-                    if (kt >= kt0) {
-                        if (!wait(&kv_full[s], ph, KS_TIMEOUT_SMEM_FULL)) break;
-                        if (++s == C::kStages) { s = 0; ph ^= 1u; }
-                        if (kt * kKeyTile < lo || (kt + 1) * kKeyTile > hi) {
-                            uint8_t *v = ring + vs * C::kTileBytes;
-                            for (int i = lane; i < kKeyTile * (D / 8); i += 32) {
-                                const int row = i / (D / 8), c = i % (D / 8), key = kt * kKeyTile + row;
-                                if (key < lo || key >= hi)
-                                    *reinterpret_cast<uint4 *>(v + (c / 8) * kSlabBytes + row * 128 + (c % 8) * 16) =
-                                        make_uint4(0, 0, 0, 0);
-                            }
-                            fence_proxy_async_smem();
-                            __syncwarp();
-                        }
-                    }
-                    const int ks = s;
-                    if (kt + 1 < kt1) {
-                        if (!wait(&kv_full[s], ph, KS_TIMEOUT_SMEM_FULL)) break;
-                        if (++s == C::kStages) { s = 0; ph ^= 1u; }
-                    }
-                    for (int rtile = 0; rtile < tiles; ++rtile) {
+            // ---- products, all issued by one thread
+            if (elect_one()) {
+                constexpr uint32_t idesc_s = idesc_f16<T>(kKeyTile, 0), idesc_o = idesc_f16<T>(D, 1);
+                const uint64_t q_desc = umma_smem_desc_k128(smem_u32(smem)), k_desc = umma_smem_desc_k128(smem_u32(ring));
+                const uint64_t v_desc = smem_desc_mn128(smem_u32(ring));
+                int s = 0;
+                uint32_t ph = 0, q_ph = 0, p_ph = 0;  // q_ph, p_ph: bit x is the parity of row tile x's barriers
+                for (long long x = x0; x < x1;) {
+                    int kt0, kt1;
+                    const long long upto = run_part<kChunkExtra>(it, x, x1, kt0, kt1);
+                    if (kt0 == kt1) break;  // the run ends within the item's EXTRA part: its tiles are the next CTA's
+                    const int tiles = it.rows - it.rt * kChunkRows > 128 ? 2 : 1;
+                    bool ok = true;
+                    for (int kt = kt0 - 1; kt < kt1; ++kt) {
+                        // V of tile kt and K of tile kt + 1 are the next two stages of the ring
+                        const int vs = s;
                         if (kt >= kt0) {
-                            if (!wait(&p_ready[rtile], (p_ph >> rtile) & 1u, KS_TIMEOUT_SOFTMAX)) break;
-                            p_ph ^= 1u << rtile;
-                            tc_fence_after_sync();
-                            if (lane == 0) {
-                                const uint64_t vd = smem_desc_mn128(smem_u32(ring + vs * C::kTileBytes));
-#pragma unroll
-                                for (int k = 0; k < kKeyTile / 16; ++k)
-                                    umma_f16_ts(tmem_o + rtile * D, tmem + rtile * kKeyTile + k * 8,
-                                                vd + (uint64_t)(k * (2048 >> 4)), idesc_o, kt != kt0 || k != 0);
-                                if (kt + 1 == kt1) umma_commit(&o_full[rtile]);
-                            }
-                            __syncwarp();
-                        } else {
-                            if (!wait(&q_ready[rtile], (q_ph >> rtile) & 1u, KS_TIMEOUT_SMEM_FULL)) break;
-                            q_ph ^= 1u << rtile;
-                            tc_fence_after_sync();
+                            ok = wait_bounded(kv_full + 8 * s, ph, wctx, KS_TIMEOUT_SMEM_FULL);
+                            if (++s == C::kStages) { s = 0; ph ^= 1u; }
                         }
-                        // the products of one CTA execute in the order of their issue, so S_x is written over P_x only
-                        // after the product that reads P_x
-                        if (kt + 1 < kt1) scores(rtile, ks);
+                        const int ks = s;
+                        if (kt + 1 < kt1 && ok) {
+                            ok = wait_bounded(kv_full + 8 * s, ph, wctx, KS_TIMEOUT_SMEM_FULL);
+                            if (++s == C::kStages) { s = 0; ph ^= 1u; }
+                        }
+                        if (!ok) break;
+#pragma unroll 1
+                        for (int r = 0; r < tiles; ++r) {
+                            if (kt >= kt0) {
+                                const uint64_t vd = v_desc + (uint64_t)(vs * (C::kTileBytes >> 4));
+                                const uint32_t par = (p_ph >> r) & 1u;
+                                ok = wait_bounded(p_ready + 16 * r, par, wctx, KS_TIMEOUT_SOFTMAX);
+                                if (!ok) break;
+                                tc_fence_after_sync();
+                                umma_f16_ts4(tmem_o + r * D, tmem + r * kKeyTile, vd, idesc_o, kt != kt0);
+                                ok = wait_bounded(p_ready + 16 * r + 8, par, wctx, KS_TIMEOUT_SOFTMAX);
+                                if (!ok) break;
+                                tc_fence_after_sync();
+                                umma_f16_ts4(tmem_o + r * D, tmem + r * kKeyTile + 32, vd + (64 * 128 >> 4), idesc_o, 1u);
+                                p_ph ^= 1u << r;
+                                if (kt + 1 == kt1) commit_to(o_full + 8 * r);
+                            } else {
+                                ok = wait_bounded(q_ready + 8 * r, (q_ph >> r) & 1u, wctx, KS_TIMEOUT_SOFTMAX);
+                                if (!ok) break;
+                                q_ph ^= 1u << r;
+                                tc_fence_after_sync();
+                            }
+                            // the products of one CTA execute in the order of their issue, so scores are written over weights
+                            // only after the product that reads these
+                            if (kt + 1 < kt1) {
+                                const uint64_t qd = q_desc + (uint64_t)(r * (C::kTileBytes >> 4));
+                                const uint64_t kd = k_desc + (uint64_t)(ks * (C::kTileBytes >> 4));
+#pragma unroll
+                                for (int d = 0; d < D / 64; ++d)
+                                    umma_f16_ss4(tmem + r * kKeyTile, qd + (uint64_t)(d * (kSlabBytes >> 4)),
+                                                 kd + (uint64_t)(d * (kSlabBytes >> 4)), idesc_s, d != 0);
+                                commit_to(s_full + 8 * r);
+                            }
+                        }
+                        if (!ok) break;
+                        if (kt >= kt0) commit_to(kv_empty + 8 * vs);
+                        if (kt + 1 < kt1) commit_to(kv_empty + 8 * ks);
                     }
                     if (!ok) break;
-                    if (lane == 0) {
-                        if (kt >= kt0) umma_commit(&kv_empty[vs]);
-                        if (kt + 1 < kt1) umma_commit(&kv_empty[ks]);
-                    }
-                    __syncwarp();
-                }
-                x = min(x1, end);
-                if (x < x1) {
-                    __syncwarp();
-                    if (lane == 0) next_item<kChunkRows, kKeyTile>(a, it);
-                    __syncwarp();
+                    x = upto;
+                    if (x < x1) next_item<kChunkRows, kKeyTile, kChunkExtra>(a, it);
                 }
             }
+            __syncwarp();
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
@@ -300,135 +410,193 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const int tile = warp >> 2, sub = warp & 3;
         const uint32_t lanes = (uint32_t)(sub * 32) << 16;
         const uint32_t ts = tmem + lanes + tile * kKeyTile, to = tmem_o + lanes + tile * D;
-        uint32_t s_ph = 0, o_ph = 0;
-        bool ok = true;
-        for (long long x = x0; ok && x < x1;) {
-            const long long end = it.begin + (it.kt1 - it.kt0);
-            const int kt0 = it.kt0 + (int)(x - it.begin), kt1 = it.kt0 + (int)(min(x1, end) - it.begin);
-            const int row0 = it.rt * kChunkRows + tile * 128;
-            if (row0 < it.rows) {
-                const int r = row0 + sub * 32 + lane;
-                const bool live = r < it.rows;
-                const int tok = live ? r / a.group : 0, head = it.h * a.group + (live ? r % a.group : 0);
-                int lo = 0, hi = 0x7fffffff;  // a row that is not there masks nothing
-                if (live) visible_keys(a, it.seq.keys - it.seq.n + tok, it.seq.keys, lo, hi);
-                const int lo_max = __reduce_max_sync(0xffffffffu, lo), hi_min = __reduce_min_sync(0xffffffffu, hi);
-                {  // the row's queries, in the swizzled K-major layout
-                    const uint4 *src = reinterpret_cast<const uint4 *>(
-                        reinterpret_cast<const T *>(a.q) + (long long)(it.seq.q0 + tok) * a.q_ts + head * a.q_hs);
-                    const int rr = sub * 32 + lane;
-                    uint8_t *dst = smem + tile * C::kTileBytes + rr * 128;
+        constexpr int kChunks = D / 8;          // 16-byte chunks of a row
+        constexpr int kRowsPerPass = 32 / kChunks;
+        // The warp's 32 rows of shared memory: queries in the swizzled K-major layout, and after a run the way of its results
+        // to memory.  Global memory is accessed kRowsPerPass whole rows at a time.
+        uint8_t *mine = smem + tile * C::kTileBytes + sub * 32 * 128;
+        auto chunk_at = [&](int row, int c) { return mine + (c / 8) * kSlabBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4); };
+        const int pass_row = lane / kChunks, pass_chunk = lane % kChunks;
+        auto q_at = [&](int r) {
+            const int tok = a.by_group.div(r), head = it.h * a.group + r - tok * a.group;
+            return reinterpret_cast<const T *>(a.q) + (it.seq.q0 + tok) * a.q_ts + head * a.q_hs + pass_chunk * 8;
+        };
+        auto load_q = [&](int row0) {
+            uint4 qv[kChunks];
 #pragma unroll
-                    for (int c = 0; c < D / 8; ++c)
-                        *reinterpret_cast<uint4 *>(dst + (c / 8) * kSlabBytes + (((c & 7) ^ (rr & 7)) << 4)) =
-                            live ? src[c] : make_uint4(0, 0, 0, 0);
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&q_ready[tile]);
-                }
-                float m = -INFINITY, l = 0.0f;
+            for (int i = 0; i < kChunks; ++i) {
+                const int r = row0 + i * kRowsPerPass + pass_row;
+                qv[i] = make_uint4(0, 0, 0, 0);
+                if (r < it.rows) qv[i] = *reinterpret_cast<const uint4 *>(q_at(r));
+            }
+#pragma unroll
+            for (int i = 0; i < kChunks; ++i)
+                *reinterpret_cast<uint4 *>(chunk_at(i * kRowsPerPass + pass_row, pass_chunk)) = qv[i];
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) arrive_on(q_ready + 8 * tile);
+        };
+        uint32_t s_ph = 0, o_ph = 0;
+        int v_stage = 1, v_ph = 0;  // of the ring, and its parity: where the values of the current tile arrive
+        bool ok = true, first_run = true;
+        for (long long x = x0; x < x1;) {
+            int kt0, kt1;
+            long long upto = run_part<kChunkExtra>(it, x, x1, kt0, kt1);
+            if (kt0 == kt1) break;  // the run ends within the item's EXTRA part: its tiles are the next CTA's
+            const int row0 = it.rt * kChunkRows + tile * 128 + sub * 32;
+            const bool active = it.rt * kChunkRows + tile * 128 < it.rows;
+            float m = -INFINITY, l = 0.0f;
+            const int item_lo = it.lo, item_hi = it.hi;
+            if (active) {
+                if (first_run) load_q(row0);
+                int lo = 0, hi = 0x7fffffff;  // a row that is not there masks nothing
+                if (row0 + lane < it.rows)
+                    visible_keys(a, it.seq.keys - it.seq.n + a.by_group.div(row0 + lane), it.seq.keys, lo, hi);
+                const int lo_max = __reduce_max_sync(0xffffffffu, lo), hi_min = __reduce_min_sync(0xffffffffu, hi);
                 for (int kt = kt0; kt < kt1; ++kt) {
-                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_full[tile], s_ph, wctx, KS_TIMEOUT_SOFTMAX));
+                    ok = __all_sync(0xffffffffu, wait_bounded(s_full + 8 * tile, s_ph, wctx, KS_TIMEOUT_SOFTMAX));
                     if (!ok) break;
                     s_ph ^= 1u;
                     tc_fence_after_sync();
-                    // scores are read twice, first for the maximum, then for the weights: 128 fp32 registers less, for
-                    // 64 KB of tensor-memory reads per tile
+                    if (tile == 0) {
+                        // Values of keys that the item's rows do not see may be anything, NaN too, and 0 x NaN is no zero: the
+                        // four warps of tile A clear them before their weights let the products of this tile begin
+                        if (kt * kKeyTile < item_lo || (kt + 1) * kKeyTile > item_hi) {
+                            ok = __all_sync(0xffffffffu, wait_bounded(kv_full + 8 * v_stage, v_ph, wctx, KS_TIMEOUT_SMEM_FULL));
+                            if (!ok) break;
+                            uint8_t *v = ring + v_stage * C::kTileBytes;
+                            for (int row = sub * 32 + lane / 8; row < sub * 32 + 32; row += 4) {
+                                const int key = kt * kKeyTile + row;
+                                if (key < item_lo || key >= item_hi) {
+#pragma unroll
+                                    for (int d = 0; d < D / 64; ++d)
+                                        *reinterpret_cast<uint4 *>(v + d * kSlabBytes + row * 128 + (lane & 7) * 16) =
+                                            make_uint4(0, 0, 0, 0);
+                                }
+                            }
+                            fence_proxy_async_smem();
+                        }
+                        v_stage += 2;
+                        if (v_stage >= C::kStages) { v_stage -= C::kStages; v_ph ^= 1; }
+                    }
+                    uint32_t s[4][32];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tmem_ld_32x32(ts + 32 * c, s[c]);
+                    tmem_ld_wait();
+                    auto f = [&](int i) { return __uint_as_float(s[i / 32][i % 32]); };
                     const int key0 = kt * kKeyTile;
                     const bool edge = key0 < lo_max || key0 + kKeyTile > hi_min;
-                    auto hide = [&](uint32_t(&s)[32], int c) {
-                        if (!edge) return;
+                    if (edge) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const int key = key0 + 32 * c + i;
-                            if (key < lo || key >= hi) s[i] = 0xff800000u;
-                        }
-                    };
-                    uint32_t s[2][32];
-                    float top = -INFINITY;
-                    tmem_ld_32x32(ts, s[0]);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        tmem_ld_wait();
-                        tmem_ld_32x32(ts + 32 * ((c + 1) & 3), s[(c + 1) & 1]);  // the last one is the first of the second pass
-                        hide(s[c & 1], c);
-                        float t4[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) t4[i] = __uint_as_float(s[c & 1][i]);
-#pragma unroll
-                        for (int i = 4; i < 32; ++i) t4[i & 3] = fmaxf(t4[i & 3], __uint_as_float(s[c & 1][i]));
-                        top = fmaxf(top, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])));
+                        for (int i = 0; i < kKeyTile; ++i)
+                            if (key0 + i < lo || key0 + i >= hi) s[i / 32][i % 32] = 0xff800000u;
                     }
+                    float t8[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        t8[i] = f(i);
+#pragma unroll
+                        for (int j = 8; j < kKeyTile - 8; j += 16) t8[i] = max3(t8[i], f(i + j), f(i + j + 8));
+                        t8[i] = fmaxf(t8[i], f(i + kKeyTile - 8));
+                    }
+                    const float top = max3(max3(t8[0], t8[1], t8[2]), max3(t8[3], t8[4], t8[5]), fmaxf(t8[6], t8[7]));
                     if (kt == kt0) {
                         m = top;
                     } else if (__any_sync(0xffffffffu, (top - m) * a.scale_log2 > kLazyRescale)) {
                         const float mn = fmaxf(m, top);
-                        const float f = m == -INFINITY ? 0.0f : fast_ex2((m - mn) * a.scale_log2);
+                        const float g = m == -INFINITY ? 0.0f : fast_ex2((m - mn) * a.scale_log2);
                         m = mn;
-                        l *= f;
+                        l *= g;
 #pragma unroll
-                        for (int c = 0; c < D / 32; ++c) {
-                            uint32_t o[32];
-                            tmem_ld_32x32(to + 32 * c, o);
+                        for (int c = 0; c < D / 16; ++c) {
+                            uint32_t o[16];
+                            tmem_ld_32x16(to + 16 * c, o);
                             tmem_ld_wait();
-                            uint32_t u[2][16];
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) u[i / 16][i % 16] = __float_as_uint(__uint_as_float(o[i]) * f);
-                            tmem_st_32x16(to + 32 * c, u[0]);
-                            tmem_st_32x16(to + 32 * c + 16, u[1]);
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * g);
+                            tmem_st_32x16(to + 16 * c, o);
                         }
                     }
                     const float ref = m == -INFINITY ? 0.0f : m * a.scale_log2;
-                    float sum[4] = {};
+                    const uint64_t scale2 = pair2(a.scale_log2, a.scale_log2), ref2 = pair2(-ref, -ref);
+                    uint64_t sum[4] = {};
+                    // weights of 32 keys at a time over the scores, which are in registers by now.  POLY of 8 pairs go to the
+                    // multiply-add pipe, the others to the special-function unit, which alone would bound the kernel.
+                    auto weights = [&](auto poly) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        tmem_ld_wait();
-                        if (c < 3) tmem_ld_32x32(ts + 32 * (c + 1), s[(c + 1) & 1]);
-                        hide(s[c & 1], c);
-                        uint32_t w[16];
+                        for (int c = 0; c < 4; ++c) {
+                            uint32_t w[16];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float e0 = fast_ex2(fmaf(__uint_as_float(s[c & 1][2 * i]), a.scale_log2, -ref));
-                            const float e1 = fast_ex2(fmaf(__uint_as_float(s[c & 1][2 * i + 1]), a.scale_log2, -ref));
-                            sum[(2 * i) & 3] += e0;
-                            sum[(2 * i + 1) & 3] += e1;
-                            w[i] = Half2Of<T>::pack(e0, e1);
+                            for (int i = 0; i < 16; ++i) {
+                                const uint64_t v = fma2(pair2(f(32 * c + 2 * i), f(32 * c + 2 * i + 1)), scale2, ref2);
+                                float e0, e1;
+                                if ((i & 7) < decltype(poly)::value) {
+                                    poly_ex2<IsBf16<T>::value ? 3 : 4>(v, e0, e1);
+                                } else {
+                                    unpair2(v, e0, e1);
+                                    e0 = fast_ex2(e0);
+                                    e1 = fast_ex2(e1);
+                                }
+                                sum[i & 3] = add2(sum[i & 3], pair2(e0, e1));
+                                w[i] = Half2Of<T>::pack(e0, e1);
+                            }
+                            tmem_st_32x16(ts + 16 * c, w);
+                            if (c & 1) {  // half of the weights: their product may begin
+                                tmem_st_wait();
+                                tc_fence_before_sync();
+                                __syncwarp();
+                                if (lane == 0) arrive_on(p_ready + 16 * tile + 8 * (c / 2));
+                            }
                         }
-                        // columns 16 c: scores that have been read already
-                        tmem_st_32x16(ts + 16 * c, w);
-                    }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    tmem_st_wait();
-                    tc_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_ready[tile]);
-                }
-                if (ok) {
-                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&o_full[tile], o_ph, wctx, KS_TIMEOUT_TMEM_FULL));
-                    o_ph ^= 1u;
+                    };
+                    // hidden keys need weights of exactly zero, which the polynomial does not give
+                    if (edge) weights(Int<0>());
+                    else weights(Int<kPolyPairs<D>>());
+                    float l0, l1;
+                    unpair2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), l0, l1);
+                    l += l0 + l1;
                 }
                 if (!ok) break;
+            }
+            // what the end of this run needs, then on to the next item, whose queries come to L2 meanwhile
+            const long long begin = it.begin + kChunkExtra;
+            const int first = map.run_of(begin), final = map.run_of(begin + (it.kt1 - it.kt0) - 1);
+            const int rows = it.rows, head0 = it.h * a.group, q0 = it.seq.q0;
+            x = upto;
+            bool more = false;
+            if (x < x1) {
+                __syncwarp();
+                if (lane == 0) next_item<kChunkRows, kKeyTile, kChunkExtra>(a, it);
+                __syncwarp();
+                int n0, n1;
+                run_part<kChunkExtra>(it, x, x1, n0, n1);
+                more = n0 != n1 && it.rt * kChunkRows + tile * 128 < it.rows;
+                const int r = it.rt * kChunkRows + tile * 128 + sub * 32 + lane;
+                if (more && r < it.rows) {
+#pragma unroll
+                    for (int d = 0; d < D; d += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(q_at(r) - pass_chunk * 8 + d));
+                }
+            }
+            first_run = false;
+            if (active) {
+                ok = __all_sync(0xffffffffu, wait_bounded(o_full + 8 * tile, o_ph, wctx, KS_TIMEOUT_TMEM_FULL));
+                if (!ok) break;
+                o_ph ^= 1u;
                 tc_fence_after_sync();
-                const int first = run_of(it.begin, total, runs), final = run_of(end - 1, total, runs);
-                T *dst = reinterpret_cast<T *>(a.out) + (long long)(it.seq.q0 + tok) * a.o_ts + head * a.o_hs;
-                if (first == final) {
-                    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+                bool write = first == final;
+                float inv = l > 0.0f ? 1.0f / l : 0.0f;
+                if (write) {
 #pragma unroll
                     for (int c = 0; c < D / 32; ++c) {
                         uint32_t o[32];
                         tmem_ld_32x32(to + 32 * c, o);
                         tmem_ld_wait();
-                        if (live) {
+                        auto g = [&](int i) { return __uint_as_float(o[i]) * inv; };
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                uint32_t p[4];
-#pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    p[e] = Half2Of<T>::pack(__uint_as_float(o[8 * i + 2 * e]) * inv,
-                                                            __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
-                                *reinterpret_cast<uint4 *>(dst + 32 * c + 8 * i) = make_uint4(p[0], p[1], p[2], p[3]);
-                            }
-                        }
+                        for (int i = 0; i < 4; ++i)
+                            *reinterpret_cast<uint4 *>(chunk_at(lane, 4 * c + i)) =
+                                make_uint4(Half2Of<T>::pack(g(8 * i), g(8 * i + 1)), Half2Of<T>::pack(g(8 * i + 2), g(8 * i + 3)),
+                                           Half2Of<T>::pack(g(8 * i + 4), g(8 * i + 5)), Half2Of<T>::pack(g(8 * i + 6), g(8 * i + 7)));
                     }
                 } else {
                     // [slot of the CTA][warp]: columns in vectors of four, 32 rows each
@@ -451,14 +619,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     __threadfence();
                     __syncwarp();
                     int before = 0;
-                    int *ticket = a.tickets + first * 8 + warp;
                     if (lane == 0) {
+                        int *ticket = a.tickets + first * 8 + warp;
                         before = atomicAdd(ticket, 1);
                         if (before == final - first) *ticket = 0;  // zero again for the next launch
                     }
                     before = __shfl_sync(0xffffffffu, before, 0);
                     __threadfence();
-                    if (before == final - first) {
+                    write = before == final - first;
+                    if (write) {  // the last of the item's CTAs joins the parts, in the order of their keys
                         float top = -INFINITY, sum = 0.0f;
                         for (int cta = first; cta <= final; ++cta) top = fmaxf(top, __ldcg(part_of(cta) + 32 * D + lane));
                         const float ref = top == -INFINITY ? 0.0f : top;
@@ -466,35 +635,52 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                             const float *pc = part_of(cta) + 32 * D + lane;
                             sum = fmaf(__ldcg(pc + 32), fast_ex2((__ldcg(pc) - ref) * a.scale_log2), sum);
                         }
-                        const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+                        inv = sum > 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll 1
-                        for (int c = 0; c < D / 8; ++c) {
-                            float v[8] = {};
+                        for (int c = 0; c < D / 32; ++c) {
+                            float v[32] = {};
+#pragma unroll 1
                             for (int cta = first; cta <= final; ++cta) {
                                 const float *pc = part_of(cta);
-                                const float f = fast_ex2((__ldcg(pc + 32 * D + lane) - ref) * a.scale_log2);
-                                const float4 u0 = __ldcg(reinterpret_cast<const float4 *>(pc + ((2 * c) * 32 + lane) * 4));
-                                const float4 u1 = __ldcg(reinterpret_cast<const float4 *>(pc + ((2 * c + 1) * 32 + lane) * 4));
-                                v[0] = fmaf(u0.x, f, v[0]); v[1] = fmaf(u0.y, f, v[1]);
-                                v[2] = fmaf(u0.z, f, v[2]); v[3] = fmaf(u0.w, f, v[3]);
-                                v[4] = fmaf(u1.x, f, v[4]); v[5] = fmaf(u1.y, f, v[5]);
-                                v[6] = fmaf(u1.z, f, v[6]); v[7] = fmaf(u1.w, f, v[7]);
+                                const float g = fast_ex2((__ldcg(pc + 32 * D + lane) - ref) * a.scale_log2);
+                                float4 u[8];
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) u[i] = __ldcg(reinterpret_cast<const float4 *>(pc) + (8 * c + i) * 32 + lane);
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) {
+                                    v[4 * i] = fmaf(u[i].x, g, v[4 * i]);
+                                    v[4 * i + 1] = fmaf(u[i].y, g, v[4 * i + 1]);
+                                    v[4 * i + 2] = fmaf(u[i].z, g, v[4 * i + 2]);
+                                    v[4 * i + 3] = fmaf(u[i].w, g, v[4 * i + 3]);
+                                }
                             }
-                            if (live)
-                                *reinterpret_cast<uint4 *>(dst + 8 * c) =
-                                    make_uint4(Half2Of<T>::pack(v[0] * inv, v[1] * inv), Half2Of<T>::pack(v[2] * inv, v[3] * inv),
-                                               Half2Of<T>::pack(v[4] * inv, v[5] * inv), Half2Of<T>::pack(v[6] * inv, v[7] * inv));
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                *reinterpret_cast<uint4 *>(chunk_at(lane, 4 * c + i)) = make_uint4(
+                                    Half2Of<T>::pack(v[8 * i] * inv, v[8 * i + 1] * inv),
+                                    Half2Of<T>::pack(v[8 * i + 2] * inv, v[8 * i + 3] * inv),
+                                    Half2Of<T>::pack(v[8 * i + 4] * inv, v[8 * i + 5] * inv),
+                                    Half2Of<T>::pack(v[8 * i + 6] * inv, v[8 * i + 7] * inv));
                         }
                     }
                 }
+                if (write) {
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < kChunks; ++i) {
+                        const int row = i * kRowsPerPass + pass_row, r = row0 + row;
+                        const uint4 v = *reinterpret_cast<const uint4 *>(chunk_at(row, pass_chunk));
+                        if (r < rows) {
+                            const int tok = a.by_group.div(r), head = head0 + r - tok * a.group;
+                            *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + (q0 + tok) * a.o_ts + head * a.o_hs +
+                                                       pass_chunk * 8) = v;
+                        }
+                    }
+                    __syncwarp();
+                }
                 tc_fence_before_sync();  // O has been read before the next run's first product, which waits for p_ready
             }
-            x = min(x1, end);
-            if (x < x1) {
-                __syncwarp();
-                if (lane == 0) next_item<kChunkRows, kKeyTile>(a, it);
-                __syncwarp();
-            }
+            if (more) load_q(it.rt * kChunkRows + tile * 128 + sub * 32);
         }
     }
 
