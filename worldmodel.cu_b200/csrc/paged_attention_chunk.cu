@@ -132,27 +132,31 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return r;
 }
 // 2^x for x in [-inf, 2^22) on the multiply-add pipe: x = n + f, n the nearest integer, |f| <= 1/2; 2^f by the polynomial of
-// least relative error over that interval (degree 3: 7.5e-5, for weights rounded to bf16 by up to 2^-9; degree 4: 2.6e-6,
-// for fp16's 2^-12), n added to the exponent.  Results below 2^-126 become about 2^-126.
+// least relative error over that interval among those that are exact at 0 (degree 3: 1.0e-4, for weights rounded to bf16 by
+// up to 2^-9; degree 4: 2.8e-6, for fp16's 2^-12), n added to the exponent.  x <= -127, -inf too, gives exactly 0.
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 template <int DEGREE>
 __device__ __forceinline__ void poly_ex2(uint64_t x, float &e0, float &e1) {
     float a, b;
     unpair2(x, a, b);
-    x = pair2(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+    x = pair2(max_nan(a, -127.0f), max_nan(b, -127.0f));
     const float magic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer in the low bits
-    const uint64_t t = add2(x, pair2(magic, magic));
+    const uint64_t one = pair2(1.0f, 1.0f), t = add2(x, pair2(magic, magic));
     const uint64_t f = fma2(add2(t, pair2(-magic, -magic)), pair2(-1.0f, -1.0f), x);
     uint64_t p;
     if (DEGREE == 3) {
-        p = fma2(pair2(0.05517132207751274f, 0.05517132207751274f), f, pair2(0.2426113337278366f, 0.2426113337278366f));
-        p = fma2(p, f, pair2(0.6932610869407654f, 0.6932610869407654f));
-        p = fma2(p, f, pair2(0.9999280571937561f, 0.9999280571937561f));
+        p = fma2(pair2(0.05500893294811249f, 0.05500893294811249f), f, pair2(0.2422109693288803f, 0.2422109693288803f));
+        p = fma2(p, f, pair2(0.6932829022407532f, 0.6932829022407532f));
     } else {
-        p = fma2(pair2(0.00957053154706955f, 0.00957053154706955f), f, pair2(0.05591866374015808f, 0.05591866374015808f));
-        p = fma2(p, f, pair2(0.24024735391139984f, 0.24024735391139984f));
-        p = fma2(p, f, pair2(0.6931216716766357f, 0.6931216716766357f));
-        p = fma2(p, f, pair2(0.9999992847442627f, 0.9999992847442627f));
+        p = fma2(pair2(0.009585382416844368f, 0.009585382416844368f), f, pair2(0.05590662732720375f, 0.05590662732720375f));
+        p = fma2(p, f, pair2(0.24024038016796112f, 0.24024038016796112f));
+        p = fma2(p, f, pair2(0.6931241750717163f, 0.6931241750717163f));
     }
+    p = fma2(p, f, one);
     float p0, p1, t0, t1;
     unpair2(p, p0, p1);
     unpair2(t, t0, t1);
@@ -180,10 +184,6 @@ __host__ __device__ constexpr uint32_t idesc_f16(int n, uint32_t b_mn_major) {
            ((uint32_t)(128 >> 4) << 24);
 }
 
-template <int N>
-struct Int {
-    static constexpr int value = N;
-};
 // Of every 8 pairs of weights, how many the multiply-add pipe computes.
 template <int D>
 constexpr int kPolyPairs = D == 128 ? 2 : 4;
@@ -201,7 +201,7 @@ __device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
     return ok != 0;
 }
 __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, const WaitCtx &w, int code) {
-    if (try_wait(bar, parity)) return true;
+    if (__builtin_expect(try_wait(bar, parity), 1)) return true;
     const unsigned long long t0 = global_timer_ns();
     uint32_t spins = 0;
     while (!try_wait(bar, parity)) {
@@ -365,14 +365,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                             if (kt >= kt0) {
                                 const uint64_t vd = v_desc + (uint64_t)(vs * (C::kTileBytes >> 4));
                                 const uint32_t par = (p_ph >> r) & 1u;
-                                ok = wait_bounded(p_ready + 16 * r, par, wctx, KS_TIMEOUT_SOFTMAX);
+#pragma unroll 1
+                                for (int half = 0; half < 2; ++half) {
+                                    ok = wait_bounded(p_ready + 16 * r + 8 * half, par, wctx, KS_TIMEOUT_SOFTMAX);
+                                    if (!ok) break;
+                                    tc_fence_after_sync();
+                                    umma_f16_ts4(tmem_o + r * D, tmem + r * kKeyTile + 32 * half,
+                                                 vd + (uint64_t)(half * (64 * 128 >> 4)), idesc_o, kt != kt0 || half);
+                                }
                                 if (!ok) break;
-                                tc_fence_after_sync();
-                                umma_f16_ts4(tmem_o + r * D, tmem + r * kKeyTile, vd, idesc_o, kt != kt0);
-                                ok = wait_bounded(p_ready + 16 * r + 8, par, wctx, KS_TIMEOUT_SOFTMAX);
-                                if (!ok) break;
-                                tc_fence_after_sync();
-                                umma_f16_ts4(tmem_o + r * D, tmem + r * kKeyTile + 32, vd + (64 * 128 >> 4), idesc_o, 1u);
                                 p_ph ^= 1u << r;
                                 if (kt + 1 == kt1) commit_to(o_full + 8 * r);
                             } else {
@@ -520,38 +521,33 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     const float ref = m == -INFINITY ? 0.0f : m * a.scale_log2;
                     const uint64_t scale2 = pair2(a.scale_log2, a.scale_log2), ref2 = pair2(-ref, -ref);
                     uint64_t sum[4] = {};
-                    // weights of 32 keys at a time over the scores, which are in registers by now.  POLY of 8 pairs go to the
+                    // weights of 32 keys at a time over the scores, which are in registers by now.  Some pairs go to the
                     // multiply-add pipe, the others to the special-function unit, which alone would bound the kernel.
-                    auto weights = [&](auto poly) {
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            uint32_t w[16];
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t w[16];
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                const uint64_t v = fma2(pair2(f(32 * c + 2 * i), f(32 * c + 2 * i + 1)), scale2, ref2);
-                                float e0, e1;
-                                if ((i & 7) < decltype(poly)::value) {
-                                    poly_ex2<IsBf16<T>::value ? 3 : 4>(v, e0, e1);
-                                } else {
-                                    unpair2(v, e0, e1);
-                                    e0 = fast_ex2(e0);
-                                    e1 = fast_ex2(e1);
-                                }
-                                sum[i & 3] = add2(sum[i & 3], pair2(e0, e1));
-                                w[i] = Half2Of<T>::pack(e0, e1);
+                        for (int i = 0; i < 16; ++i) {
+                            const uint64_t v = fma2(pair2(f(32 * c + 2 * i), f(32 * c + 2 * i + 1)), scale2, ref2);
+                            float e0, e1;
+                            if ((i & 7) < kPolyPairs<D>) {
+                                poly_ex2<IsBf16<T>::value ? 3 : 4>(v, e0, e1);
+                            } else {
+                                unpair2(v, e0, e1);
+                                e0 = fast_ex2(e0);
+                                e1 = fast_ex2(e1);
                             }
-                            tmem_st_32x16(ts + 16 * c, w);
-                            if (c & 1) {  // half of the weights: their product may begin
-                                tmem_st_wait();
-                                tc_fence_before_sync();
-                                __syncwarp();
-                                if (lane == 0) arrive_on(p_ready + 16 * tile + 8 * (c / 2));
-                            }
+                            sum[i & 3] = add2(sum[i & 3], pair2(e0, e1));
+                            w[i] = Half2Of<T>::pack(e0, e1);
                         }
-                    };
-                    // hidden keys need weights of exactly zero, which the polynomial does not give
-                    if (edge) weights(Int<0>());
-                    else weights(Int<kPolyPairs<D>>());
+                        tmem_st_32x16(ts + 16 * c, w);
+                        if (c & 1) {  // half of the weights: their product may begin
+                            tmem_st_wait();
+                            tc_fence_before_sync();
+                            __syncwarp();
+                            if (lane == 0) arrive_on(p_ready + 16 * tile + 8 * (c / 2));
+                        }
+                    }
                     float l0, l1;
                     unpair2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), l0, l1);
                     l += l0 + l1;
