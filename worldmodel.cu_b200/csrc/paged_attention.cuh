@@ -308,6 +308,30 @@ __device__ __forceinline__ long long run_part(const Item &it, long long x, long 
     return upto;
 }
 
+// A walk over the items of one CTA's run.
+struct Walk {
+    Item it;
+    long long x, x1, upto;  // place in the run, its end, the end of this item's part of it
+    RunMap map;
+    int kt0, kt1;           // KV tiles of the item that the run holds; none at the end of the run
+    int first, final;       // the CTAs that share the item
+    template <int EXTRA>
+    __device__ __forceinline__ void locate() {
+        kt0 = kt1 = 0;
+        if (x >= x1) return;
+        upto = run_part<EXTRA>(it, x, x1, kt0, kt1);
+        const long long begin = it.begin + EXTRA;
+        first = map.run_of(begin);
+        final = map.run_of(begin + (it.kt1 - it.kt0) - 1);
+    }
+    template <int ROWS, int KT, int EXTRA>
+    __device__ __forceinline__ void advance(const AttnParams &a) {
+        x = upto;
+        if (x < x1) next_item<ROWS, KT, EXTRA>(a, it);
+        locate<EXTRA>();
+    }
+};
+
 }  // namespace
 
 }  // namespace b200

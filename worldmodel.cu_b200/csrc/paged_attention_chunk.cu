@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     using C = ChunkCfg<D>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ PlanShared<kChunkThreads> plan;
-    __shared__ Item items[10];  // every warp's own place in the plan, kept out of the loops' registers
+    __shared__ Walk walks[10];  // every warp's own, kept out of the loops' registers
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *ring = smem + 2 * C::kTileBytes;
     // barriers: [stage] pages have landed; [stage] their products are done; [row tile] its queries are in shared memory; its
@@ -264,14 +264,21 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         tma_prefetch_desc(&tm_v);
     }
     pdl_wait();
-    long long x0, x1;
-    RunMap map;
     {
-        Item first;
-        if (!plan_run<kChunkRows, kKeyTile, kChunkExtra, kChunkThreads>(a, plan, map, x0, x1, first)) return;
-        if (lane == 0 && warp < 10) items[warp] = first;
+        Walk w;
+        if (!plan_run<kChunkRows, kKeyTile, kChunkExtra, kChunkThreads>(a, plan, w.map, w.x, w.x1, w.it)) return;
+        w.locate<kChunkExtra>();
+        if (lane == 0 && warp < 10) walks[warp] = w;
     }
-    Item &it = items[min(warp, 9)];
+    Walk &walk = walks[min(warp, 9)];
+    const volatile Walk &now = walk;
+    Item &it = walk.it;
+    // one lane takes the warp's walk to its next item
+    auto advance = [&]() {
+        __syncwarp();
+        if (lane == 0) walk.advance<kChunkRows, kKeyTile, kChunkExtra>(a);
+        __syncwarp();
+    };
     if (warp == 9) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
@@ -290,10 +297,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             uint32_t ph = 0;
             bool ok = true, drop = ex.debug_drop_load != 0;
             const int boxes = kKeyTile / ex.page_box;  // along the keys of a tile
-            for (long long x = x0; ok && x < x1;) {
-                int kt0, kt1;
-                const long long upto = run_part<kChunkExtra>(it, x, x1, kt0, kt1);
-                if (kt0 == kt1) break;  // the run ends within the item's EXTRA part: its tiles are the next CTA's
+            while (ok && now.kt0 < now.kt1) {
+                const int kt0 = now.kt0, kt1 = now.kt1;
                 const int lo = it.lo, hi = it.hi, kv_head = it.h;
                 const int *table = a.c.page_table + (long long)it.s * a.c.max_pages;
                 for (int kt = kt0; ok && kt < kt1; ++kt) {
@@ -326,12 +331,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                         if (++s == C::kStages) { s = 0; ph ^= 1u; }
                     }
                 }
-                x = upto;
-                if (x < x1) {
-                    __syncwarp();
-                    if (lane == 0) next_item<kChunkRows, kKeyTile, kChunkExtra>(a, it);
-                    __syncwarp();
-                }
+                advance();
             }
         } else if (warp == 9) {
             // ---- products, all issued by one thread
@@ -341,10 +341,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 const uint64_t v_desc = smem_desc_mn128(smem_u32(ring));
                 int s = 0;
                 uint32_t ph = 0, q_ph = 0, p_ph = 0;  // q_ph, p_ph: bit x is the parity of row tile x's barriers
-                for (long long x = x0; x < x1;) {
-                    int kt0, kt1;
-                    const long long upto = run_part<kChunkExtra>(it, x, x1, kt0, kt1);
-                    if (kt0 == kt1) break;  // the run ends within the item's EXTRA part: its tiles are the next CTA's
+                while (now.kt0 < now.kt1) {
+                    const int kt0 = now.kt0, kt1 = now.kt1;
                     const int tiles = it.rows - it.rt * kChunkRows > 128 ? 2 : 1;
                     bool ok = true;
                     for (int kt = kt0 - 1; kt < kt1; ++kt) {
@@ -399,8 +397,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                         if (kt + 1 < kt1) commit_to(kv_empty + 8 * ks);
                     }
                     if (!ok) break;
-                    x = upto;
-                    if (x < x1) next_item<kChunkRows, kKeyTile, kChunkExtra>(a, it);
+                    walk.advance<kChunkRows, kKeyTile, kChunkExtra>(a);
                 }
             }
             __syncwarp();
@@ -440,10 +437,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         uint32_t s_ph = 0, o_ph = 0;
         int v_stage = 1, v_ph = 0;  // of the ring, and its parity: where the values of the current tile arrive
         bool ok = true, first_run = true;
-        for (long long x = x0; x < x1;) {
-            int kt0, kt1;
-            long long upto = run_part<kChunkExtra>(it, x, x1, kt0, kt1);
-            if (kt0 == kt1) break;  // the run ends within the item's EXTRA part: its tiles are the next CTA's
+        while (now.kt0 < now.kt1) {
+            const int kt0 = now.kt0, kt1 = now.kt1;
             const int row0 = it.rt * kChunkRows + tile * 128 + sub * 32;
             const bool active = it.rt * kChunkRows + tile * 128 < it.rows;
             float m = -INFINITY, l = 0.0f;
@@ -555,18 +550,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 if (!ok) break;
             }
             // what the end of this run needs, then on to the next item, whose queries come to L2 meanwhile
-            const long long begin = it.begin + kChunkExtra;
-            const int first = map.run_of(begin), final = map.run_of(begin + (it.kt1 - it.kt0) - 1);
-            const int rows = it.rows, head0 = it.h * a.group, q0 = it.seq.q0;
-            x = upto;
-            bool more = false;
-            if (x < x1) {
-                __syncwarp();
-                if (lane == 0) next_item<kChunkRows, kKeyTile, kChunkExtra>(a, it);
-                __syncwarp();
-                int n0, n1;
-                run_part<kChunkExtra>(it, x, x1, n0, n1);
-                more = n0 != n1 && it.rt * kChunkRows + tile * 128 < it.rows;
+            const int first = now.first, final = now.final, rows = it.rows, head0 = it.h * a.group, q0 = it.seq.q0;
+            advance();
+            const bool more = now.kt0 < now.kt1 && it.rt * kChunkRows + tile * 128 < it.rows;
+            {
                 const int r = it.rt * kChunkRows + tile * 128 + sub * 32 + lane;
                 if (more && r < it.rows) {
 #pragma unroll
