@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attention_rows_kernel(const A
     const int g = lane >> 2, t = lane & 3;
     pdl_trigger();
     pdl_wait();
-    long long x0, x1;
+    int x0, x1;
     RunMap map;
     Item it;
     if (!plan_run<kRowTile, kRowsKeyTile, kRowsExtra, kRowsThreads>(a, plan, map, x0, x1, it)) return;
@@ -85,9 +85,9 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attention_rows_kernel(const A
     const int page_mask = (1 << a.c.page_shift) - 1;
     const T *kb = reinterpret_cast<const T *>(a.c.k), *vb = reinterpret_cast<const T *>(a.c.v);
 
-    for (long long x = x0; x < x1;) {
+    for (int x = x0; x < x1;) {
         int kt0, kt1;
-        const long long upto = run_part<kRowsExtra>(it, x, x1, kt0, kt1);
+        const int upto = run_part<kRowsExtra>(it, x, x1, kt0, kt1);
         if (kt0 == kt1) break;  // the run ends within the item's EXTRA part: its tiles are the next CTA's
         const int r0 = it.rt * kRowTile, rows = min(kRowTile, it.rows - r0);
 
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attention_rows_kernel(const A
                     make_float2(o[n][2 * r], o[n][2 * r + 1]);
         __syncthreads();
 
-        const long long begin = it.begin + kRowsExtra;
+        const int begin = it.begin + kRowsExtra;
         const int first = map.run_of(begin), final = map.run_of(begin + (it.kt1 - it.kt0) - 1);
         const bool whole = first == final;
         float *part = a.partials + (long long)(2 * blockIdx.x + ((int)blockIdx.x == first ? 1 : 0)) * C::kPartialFloats;
@@ -395,15 +395,24 @@ int paged_attention(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *b
     a.window = window;
     a.tickets = reinterpret_cast<int *>(workspace);
     a.partials = reinterpret_cast<float *>(reinterpret_cast<char *>(workspace) + kTicketBytes);
-    a.min_tiles = 4;
     int dev;
     const int sms = std::min(current_device_sms(dev), kMaxSms);
     AttnDeviceInfo &di = attn_device_info(dev);
     const bool bf = cache->dtype == B200_DT_BF16;
-    if ((long long)batch->max_new_tokens * a.group > kRowTile) {
+    // at most so many units of work; the kernels count them in 32 bits
+    auto work_fits = [&](long long row_tile, long long key_tile, long long extra) {
+        const double rows = (double)batch->n_tokens * a.group / row_tile + batch->n_seqs;
+        const double keys = (double)batch->max_pages * cache->page_tokens / key_tile + 1 + extra;
+        return rows * keys * cache->n_kv_heads < 2147483000.0;
+    };
+    if ((long long)batch->max_new_tokens * a.group > kRowTile || !work_fits(kRowTile, kRowsKeyTile, kRowsExtra)) {
+        if (!work_fits(256, 128, 3))
+            return fail("paged_attention: %d new tokens over up to %lld keys are too much for one call; pass fewer at a time",
+                        batch->n_tokens, (long long)batch->max_pages * cache->page_tokens);
         a.min_tiles = 2;
         return launch_attention_chunk(cache, a, sms, dev, stream);
     }
+    a.min_tiles = 4;
     if (cache->d_head == 64)
         return bf ? launch_rows<__nv_bfloat16, 64>(a, sms, di.attr_set[0][1], stream)
                   : launch_rows<__half, 64>(a, sms, di.attr_set[0][0], stream);

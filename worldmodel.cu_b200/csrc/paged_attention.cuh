@@ -51,24 +51,19 @@ namespace {
 constexpr int kTicketBytes = 16384;           // counters at the start of the workspace: one per warp that joins
 constexpr int kMaxSms = kTicketBytes / 4 / 8;  // eight such warps per SM
 
-// a / b for a >= 0, b > 0: the short division whenever both fit 32 bits, which all but absurd sizes do
-__device__ __forceinline__ long long div_small(long long a, long long b) {
-    if ((((unsigned long long)a | (unsigned long long)b) >> 32) == 0) return (unsigned)a / (unsigned)b;
-    return a / b;
-}
-
 // Cuts `total` units into `runs` runs of equal length, the first `rest` of them one unit longer.
 struct RunMap {
-    long long each, rest;
-    __device__ __forceinline__ void set(long long total, int runs) {
-        each = div_small(total, runs);
+    unsigned each, rest;
+    __device__ __forceinline__ void set(unsigned total, unsigned runs) {
+        each = total / runs;
         rest = total - each * runs;
     }
-    __device__ __forceinline__ long long start(int run) const { return run * each + min((long long)run, rest); }
+    __device__ __forceinline__ int start(unsigned run) const { return (int)(run * each + min(run, rest)); }
     // the run that holds unit x
-    __device__ __forceinline__ int run_of(long long x) const {
-        const long long longer = rest * (each + 1);
-        return (int)(x < longer ? div_small(x, each + 1) : rest + div_small(x - longer, each));
+    __device__ __forceinline__ int run_of(unsigned x) const {
+        const unsigned longer = rest * (each + 1);
+        const bool in = x < longer;
+        return (int)((in ? 0u : rest) + (in ? x : x - longer) / (in ? each + 1 : each));
     }
 };
 
@@ -108,71 +103,60 @@ struct Item {
     int rows;          // of the sequence: new tokens * group
     int kt0, kt1;      // KV tiles
     int lo, hi;        // keys
-    long long begin;   // where the item begins among all items, in units of tiles
+    int begin;         // where the item begins among all items, in units of tiles
 };
 
 template <int NT>
 struct PlanShared {
     long long warp_sum[NT / 32];
-    long long before;  // work before the sequence found
     Seq seq;
-    int s;
+    int s, before;  // the sequence found, and the work before it
 };
 
-// Work (for one key head, in tiles) of a sequence over all of its row tiles; every lane of the warp calls with its own.
+// Work (for one key head, in tiles) of a sequence over all of its row tiles; every lane of the warp calls with its own
+// sequence.  Those of one row tile are done first, a lane each; then the others one by one, a row tile per lane.
 template <int ROWS, int KT, int EXTRA>
-__device__ __forceinline__ long long seq_tiles(const AttnParams &a, const Seq &q) {
-    const int rows = q.n * a.group, n_rt = (rows + ROWS - 1) / ROWS;
+__device__ __forceinline__ long long seq_work(const AttnParams &a, const Seq &q) {
+    const int lane = threadIdx.x & 31, n_rt = (q.n * a.group + ROWS - 1) / ROWS;
+    unsigned many = __ballot_sync(0xffffffffu, n_rt > 1);
     long long total = 0;
-    int kt0, kt1, lo, hi;
-    if (n_rt <= 2) {
-        for (int rt = 0; rt < n_rt; ++rt) {
-            row_tile_keys(a, q, rt * ROWS, min(rows, (rt + 1) * ROWS), KT, kt0, kt1, lo, hi);
-            total += kt1 - kt0 + EXTRA;
-        }
-    }
-    // sequences of many row tiles: the warp takes them together, a row tile per lane
-    unsigned many = __ballot_sync(0xffffffffu, n_rt > 2);
-    const int lane = threadIdx.x & 31;
-    while (many) {
-        const int src = __ffs(many) - 1;
-        many &= many - 1;
+    bool single = true;
+#pragma unroll 1
+    do {
+        const int src = single ? lane : __ffs(many) - 1;
         Seq w;
         w.q0 = 0;
         w.n = __shfl_sync(0xffffffffu, q.n, src);
         w.keys = __shfl_sync(0xffffffffu, q.keys, src);
-        const int wrows = w.n * a.group, wn = (wrows + ROWS - 1) / ROWS;
+        const int rows = w.n * a.group, tiles = (rows + ROWS - 1) / ROWS;
+        const int last = single ? (tiles == 1 ? 1 : 0) : tiles;
         long long sum = 0;
-        for (int rt = lane; rt < wn; rt += 32) {
-            row_tile_keys(a, w, rt * ROWS, min(wrows, (rt + 1) * ROWS), KT, kt0, kt1, lo, hi);
+#pragma unroll 1
+        for (int rt = single ? 0 : lane; rt < last; rt += 32) {
+            int kt0, kt1, lo, hi;
+            row_tile_keys(a, w, rt * ROWS, min(rows, (rt + 1) * ROWS), KT, kt0, kt1, lo, hi);
             sum += kt1 - kt0 + EXTRA;
+        }
+        if (single) {
+            total = sum;
+            single = false;
+            continue;
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == src) total = sum;
-    }
+        many &= many - 1;
+    } while (many);
     return total;
 }
 
-// Inclusive scan of `v` over the block; *sum gets the block's total.
-template <int NT>
-__device__ __forceinline__ long long block_scan(long long v, PlanShared<NT> &sh, long long *sum) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__device__ __forceinline__ long long warp_scan(long long v) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const long long up = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += up;
     }
-    __syncthreads();  // the previous round's readers are done
-    if (lane == 31) sh.warp_sum[warp] = v;
-    __syncthreads();
-    long long all = 0;
-#pragma unroll
-    for (int w = 0; w < NT / 32; ++w) {
-        if (w < warp) v += sh.warp_sum[w];
-        all += sh.warp_sum[w];
-    }
-    *sum = all;
     return v;
 }
 
@@ -181,91 +165,97 @@ __device__ __forceinline__ void set_row_tile(const AttnParams &a, Item &it, int 
     row_tile_keys(a, it.seq, r0, min(it.rows, r0 + rows_per_tile), kt, it.kt0, it.kt1, it.lo, it.hi);
 }
 
-__device__ __forceinline__ Seq lane_seq(const AttnParams &a, int s) {
-    if (s < a.c.n_seqs) return load_seq(a.c, s);
-    return Seq{0, 0, 0};
-}
-
 // The run [x0, x1) of this CTA among all work (false when it has none), and the item that unit x0 belongs to.  All threads of
-// the block (NT) call it.
+// the block (NT) call it.  Up to 32 sequences every warp plans for itself; more are spread over the block.
 template <int ROWS, int KT, int EXTRA, int NT>
-__device__ bool plan_run(const AttnParams &a, PlanShared<NT> &sh, RunMap &map, long long &x0, long long &x1, Item &it) {
-    const int heads = a.c.n_kv_heads, lane = threadIdx.x & 31;
-    const bool few = a.c.n_seqs <= 32;  // every warp sees all sequences and works for itself: no barrier of the block
+__device__ bool plan_run(const AttnParams &a, PlanShared<NT> &sh, RunMap &map, int &x0, int &x1, Item &it) {
+    const int heads = a.c.n_kv_heads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const bool few = a.c.n_seqs <= 32;
+    const int step = few ? 32 : NT, mine_at = few ? lane : (int)threadIdx.x;
     long long per_head = 0, incl = 0, mine = 0;
-    Seq q;
-    if (few) {
-        q = lane_seq(a, lane);
-        incl = mine = seq_tiles<ROWS, KT, EXTRA>(a, q);
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long up = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += up;
-        }
-        per_head = __shfl_sync(0xffffffffu, incl, 31);
-    } else {
-        for (int base = 0; base < a.c.n_seqs; base += NT) {
-            q = lane_seq(a, base + (int)threadIdx.x);
-            mine = seq_tiles<ROWS, KT, EXTRA>(a, q);
-            long long sum;
-            incl = block_scan<NT>(mine, sh, &sum);
-            per_head += sum;
-        }
-    }
-    const long long total = per_head * heads;
-    if (total == 0) return false;
-    const int runs = (int)min((long long)gridDim.x, div_small(total + a.min_tiles - 1, a.min_tiles));
-    if ((int)blockIdx.x >= runs) return false;
-    map.set(total, runs);
-    x0 = map.start(blockIdx.x);
-    x1 = map.start(blockIdx.x + 1);
-    const long long target = x0 >> 31 ? x0 / heads : (long long)a.by_heads.div((int)x0);
-    long long at;  // work for one head before the sequence, then before the row tile
-    if (few) {
-        const int src = __ffs(__ballot_sync(0xffffffffu, mine > 0 && target < incl)) - 1;
-        it.s = src;
-        it.seq.q0 = __shfl_sync(0xffffffffu, q.q0, src);
-        it.seq.n = __shfl_sync(0xffffffffu, q.n, src);
-        it.seq.keys = __shfl_sync(0xffffffffu, q.keys, src);
-        at = __shfl_sync(0xffffffffu, incl - mine, src);
-    } else {
+    int target = -1;
+    Seq q = {0, 0, 0};
+    // first the sum over all sequences, then (target >= 0) the sequence that holds this CTA's first unit
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {
         long long before = 0;
-        for (int base = 0; base < a.c.n_seqs; base += NT) {
-            long long sum = per_head;
-            if (a.c.n_seqs > NT) {  // else this thread still holds its sequence's values
-                q = lane_seq(a, base + (int)threadIdx.x);
-                mine = seq_tiles<ROWS, KT, EXTRA>(a, q);
-                incl = block_scan<NT>(mine, sh, &sum);
+#pragma unroll 1
+        for (int base = 0; base < a.c.n_seqs; base += step) {
+            const int s = base + mine_at;
+            long long sum;
+            if (pass == 0 || a.c.n_seqs > step) {  // else this thread still holds its sequence's values
+                q = Seq{0, 0, 0};
+                if (s < a.c.n_seqs) q = load_seq(a.c, s);
+                mine = seq_work<ROWS, KT, EXTRA>(a, q);
+                incl = warp_scan(mine);
+                sum = __shfl_sync(0xffffffffu, incl, 31);
+                if (!few) {
+                    __syncthreads();  // the previous round's readers are done
+                    if (lane == 31) sh.warp_sum[warp] = incl;
+                    __syncthreads();
+                    sum = 0;
+#pragma unroll 1
+                    for (int w = 0; w < NT / 32; ++w) {
+                        if (w < warp) incl += sh.warp_sum[w];
+                        sum += sh.warp_sum[w];
+                    }
+                }
+            } else {
+                sum = per_head;
             }
-            const long long from = before + incl - mine;
-            if (mine > 0 && target >= from && target < from + mine) {
-                sh.s = base + (int)threadIdx.x;
-                sh.seq = q;
-                sh.before = from;
+            if (pass == 1) {
+                const long long from = before + incl - mine;
+                const bool here = mine > 0 && target >= from && target < from + mine;
+                if (few) {
+                    const int src = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+                    it.s = src;
+                    it.seq.q0 = __shfl_sync(0xffffffffu, q.q0, src);
+                    it.seq.n = __shfl_sync(0xffffffffu, q.n, src);
+                    it.seq.keys = __shfl_sync(0xffffffffu, q.keys, src);
+                    it.begin = __shfl_sync(0xffffffffu, (int)from, src);
+                } else if (here) {
+                    sh.s = s;
+                    sh.seq = q;
+                    sh.before = (int)from;
+                }
             }
             before += sum;
         }
+        if (pass == 0) {
+            per_head = before;
+            const long long total = per_head * heads;
+            if (total == 0) return false;
+            if (total >> 31) {  // only row starts that overlap lead here: the host checks the sizes
+                report_bad_page(a.c);
+                return false;
+            }
+            const int runs = min((int)gridDim.x, ((int)total - 1) / a.min_tiles + 1);
+            if ((int)blockIdx.x >= runs) return false;
+            map.set((unsigned)total, (unsigned)runs);
+            x0 = map.start(blockIdx.x);
+            x1 = map.start(blockIdx.x + 1);
+            target = a.by_heads.div(x0);
+        }
+    }
+    if (!few) {
         __syncthreads();
         it.s = sh.s;
         it.seq = sh.seq;
-        at = sh.before;
+        it.begin = sh.before;
     }
     it.rows = it.seq.n * a.group;
     const int n_rt = (it.rows + ROWS - 1) / ROWS;
+    int at = it.begin;  // work for one head before the row tile
     it.rt = 0;
     // the row tile within the sequence: 32 at a time, every warp for itself
+#pragma unroll 1
     for (int base = 0; n_rt > 1 && base < n_rt; base += 32) {
         int kt0, kt1, lo, hi, n = 0;
         if (base + lane < n_rt) {
             row_tile_keys(a, it.seq, (base + lane) * ROWS, min(it.rows, (base + lane + 1) * ROWS), KT, kt0, kt1, lo, hi);
             n = kt1 - kt0 + EXTRA;
         }
-        long long scan = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long up = __shfl_up_sync(0xffffffffu, scan, o);
-            if (lane >= o) scan += up;
-        }
+        const int scan = (int)warp_scan(n);
         const unsigned hit = __ballot_sync(0xffffffffu, n > 0 && target < at + scan);
         if (hit) {
             const int src = __ffs(hit) - 1;
@@ -277,8 +267,8 @@ __device__ bool plan_run(const AttnParams &a, PlanShared<NT> &sh, RunMap &map, l
     }
     set_row_tile(a, it, ROWS, KT);
     const int n = it.kt1 - it.kt0 + EXTRA;
-    it.h = (int)div_small(x0 - at * heads, n);
-    it.begin = at * heads + (long long)it.h * n;
+    it.h = (x0 - at * heads) / n;
+    it.begin = at * heads + it.h * n;
     return true;
 }
 
@@ -301,17 +291,17 @@ __device__ __forceinline__ void next_item(const AttnParams &a, Item &it) {
 
 // What the run [x, x1) holds of an item: tiles [t0, t1) of the item, none where only its EXTRA part lies in the run.
 template <int EXTRA>
-__device__ __forceinline__ long long run_part(const Item &it, long long x, long long x1, int &t0, int &t1) {
-    const long long tiles = it.begin + EXTRA, end = tiles + (it.kt1 - it.kt0), upto = min(x1, end);
-    t0 = it.kt0 + (int)max(x - tiles, 0ll);
-    t1 = it.kt0 + (int)max(upto - tiles, 0ll);
+__device__ __forceinline__ int run_part(const Item &it, int x, int x1, int &t0, int &t1) {
+    const int tiles = it.begin + EXTRA, upto = min(x1, tiles + (it.kt1 - it.kt0));
+    t0 = it.kt0 + max(x - tiles, 0);
+    t1 = it.kt0 + max(upto - tiles, 0);
     return upto;
 }
 
 // A walk over the items of one CTA's run.
 struct Walk {
     Item it;
-    long long x, x1, upto;  // place in the run, its end, the end of this item's part of it
+    int x, x1, upto;        // place in the run, its end, the end of this item's part of it
     RunMap map;
     int kt0, kt1;           // KV tiles of the item that the run holds; none at the end of the run
     int first, final;       // the CTAs that share the item
@@ -320,7 +310,7 @@ struct Walk {
         kt0 = kt1 = 0;
         if (x >= x1) return;
         upto = run_part<EXTRA>(it, x, x1, kt0, kt1);
-        const long long begin = it.begin + EXTRA;
+        const int begin = it.begin + EXTRA;
         first = map.run_of(begin);
         final = map.run_of(begin + (it.kt1 - it.kt0) - 1);
     }
