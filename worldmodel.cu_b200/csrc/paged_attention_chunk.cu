@@ -10,6 +10,7 @@
 // transposed.  Rows of V outside the sequence are zeroed in shared memory before their product, since 0 x NaN is no zero.
 #include <cuda.h>
 
+#include <algorithm>
 #include <mutex>
 
 #include "paged_attention.cuh"
@@ -184,35 +185,33 @@ __host__ __device__ constexpr uint32_t idesc_f16(int n, uint32_t b_mn_major) {
            ((uint32_t)(128 >> 4) << 24);
 }
 
-// Of every 8 pairs of weights, how many the multiply-add pipe computes.
+// Of every 8 pairs of weights, how many the multiply-add pipe computes.  Measured, 1 / 2 / 3 / 4 / 5 of 8: a frame of 512 tokens
+// over 8704 keys, d = 64: 66.3 / - / 63.5 / 68.3 / 73.1 us; a prompt of 8192 tokens, d = 128: 476 / 470 / 480 / 523 / 530 us.
 template <int D>
-constexpr int kPolyPairs = D == 128 ? 2 : 4;
+constexpr int kPolyPairs = D == 128 ? 2 : 3;
 
 // Waits and commits by shared-memory address: what stands between two products of the issuing thread is kept short.
+constexpr uint32_t kWaitNs = 20000;  // about how long one try of a wait sleeps
 __device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(bar), "r"(parity)
+        : "r"(bar), "r"(parity), "n"(kWaitNs)
         : "memory");
     return ok != 0;
 }
-__device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, const WaitCtx &w, int code) {
-    if (__builtin_expect(try_wait(bar, parity), 1)) return true;
-    const unsigned long long t0 = global_timer_ns();
-    uint32_t spins = 0;
+// Waits with a limit of tries; false when it runs out or another warp's has: *abort then holds the first code, which is
+// reported when the CTA ends.
+__device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, volatile int *abort, int tries, int code) {
+#pragma unroll 1
     while (!try_wait(bar, parity)) {
-        if (((++spins) & 0x3Fu) == 0) {
-            if (*w.abort_flag) return false;
-            if (global_timer_ns() - t0 > w.limit_ns) {
-                *w.abort_flag = 1;
-                if (w.status && *(volatile int *)w.status == 0) *(volatile int *)w.status = code;
-                __threadfence_system();
-                return false;
-            }
+        if (*abort) return false;
+        if (--tries <= 0) {
+            *abort = code;
+            return false;
         }
     }
     return true;
@@ -226,7 +225,7 @@ __device__ __forceinline__ void arrive_on(uint32_t bar) {
 
 struct ChunkExtra {
     int page_box;  // tokens per TMA box: min(page_tokens, 128)
-    unsigned long long wait_limit_ns;
+    int wait_tries;
     int debug_drop_load;
 };
 
@@ -248,7 +247,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     const uint32_t s_full = q_ready + 16, p_ready = s_full + 16, o_full = p_ready + 32;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * C::kStages + 10);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    const WaitCtx wctx{abort_flag, a.c.status, ex.wait_limit_ns};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     pdl_trigger();
@@ -317,7 +315,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     const unsigned mask = __ballot_sync(0xffffffffu, live);
                     const uint32_t bytes = (uint32_t)__popc(mask) * (uint32_t)ex.page_box * (D * 2);
                     for (int kv = 0; kv < 2; ++kv) {
-                        ok = __all_sync(0xffffffffu, wait_bounded(kv_empty + 8 * s, ph ^ 1u, wctx, KS_TIMEOUT_SMEM_EMPTY));
+                        ok = __all_sync(0xffffffffu, wait_bounded(kv_empty + 8 * s, ph ^ 1u, abort_flag, ex.wait_tries, KS_TIMEOUT_SMEM_EMPTY));
                         if (!ok) break;
                         if (lane == 0) mbar_arrive_expect_tx(bars + s, bytes);
                         __syncwarp();
@@ -349,12 +347,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                         // V of tile kt and K of tile kt + 1 are the next two stages of the ring
                         const int vs = s;
                         if (kt >= kt0) {
-                            ok = wait_bounded(kv_full + 8 * s, ph, wctx, KS_TIMEOUT_SMEM_FULL);
+                            ok = wait_bounded(kv_full + 8 * s, ph, abort_flag, ex.wait_tries, KS_TIMEOUT_SMEM_FULL);
                             if (++s == C::kStages) { s = 0; ph ^= 1u; }
                         }
                         const int ks = s;
                         if (kt + 1 < kt1 && ok) {
-                            ok = wait_bounded(kv_full + 8 * s, ph, wctx, KS_TIMEOUT_SMEM_FULL);
+                            ok = wait_bounded(kv_full + 8 * s, ph, abort_flag, ex.wait_tries, KS_TIMEOUT_SMEM_FULL);
                             if (++s == C::kStages) { s = 0; ph ^= 1u; }
                         }
                         if (!ok) break;
@@ -365,7 +363,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                                 const uint32_t par = (p_ph >> r) & 1u;
 #pragma unroll 1
                                 for (int half = 0; half < 2; ++half) {
-                                    ok = wait_bounded(p_ready + 16 * r + 8 * half, par, wctx, KS_TIMEOUT_SOFTMAX);
+                                    ok = wait_bounded(p_ready + 16 * r + 8 * half, par, abort_flag, ex.wait_tries, KS_TIMEOUT_SOFTMAX);
                                     if (!ok) break;
                                     tc_fence_after_sync();
                                     umma_f16_ts4(tmem_o + r * D, tmem + r * kKeyTile + 32 * half,
@@ -375,7 +373,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                                 p_ph ^= 1u << r;
                                 if (kt + 1 == kt1) commit_to(o_full + 8 * r);
                             } else {
-                                ok = wait_bounded(q_ready + 8 * r, (q_ph >> r) & 1u, wctx, KS_TIMEOUT_SOFTMAX);
+                                ok = wait_bounded(q_ready + 8 * r, (q_ph >> r) & 1u, abort_flag, ex.wait_tries, KS_TIMEOUT_SOFTMAX);
                                 if (!ok) break;
                                 q_ph ^= 1u << r;
                                 tc_fence_after_sync();
@@ -450,7 +448,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     visible_keys(a, it.seq.keys - it.seq.n + a.by_group.div(row0 + lane), it.seq.keys, lo, hi);
                 const int lo_max = __reduce_max_sync(0xffffffffu, lo), hi_min = __reduce_min_sync(0xffffffffu, hi);
                 for (int kt = kt0; kt < kt1; ++kt) {
-                    ok = __all_sync(0xffffffffu, wait_bounded(s_full + 8 * tile, s_ph, wctx, KS_TIMEOUT_SOFTMAX));
+                    ok = __all_sync(0xffffffffu, wait_bounded(s_full + 8 * tile, s_ph, abort_flag, ex.wait_tries, KS_TIMEOUT_SOFTMAX));
                     if (!ok) break;
                     s_ph ^= 1u;
                     tc_fence_after_sync();
@@ -458,7 +456,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                         // Values of keys that the item's rows do not see may be anything, NaN too, and 0 x NaN is no zero: the
                         // four warps of tile A clear them before their weights let the products of this tile begin
                         if (kt * kKeyTile < item_lo || (kt + 1) * kKeyTile > item_hi) {
-                            ok = __all_sync(0xffffffffu, wait_bounded(kv_full + 8 * v_stage, v_ph, wctx, KS_TIMEOUT_SMEM_FULL));
+                            ok = __all_sync(0xffffffffu, wait_bounded(kv_full + 8 * v_stage, v_ph, abort_flag, ex.wait_tries, KS_TIMEOUT_SMEM_FULL));
                             if (!ok) break;
                             uint8_t *v = ring + v_stage * C::kTileBytes;
                             for (int row = sub * 32 + lane / 8; row < sub * 32 + 32; row += 4) {
@@ -481,11 +479,21 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     tmem_ld_wait();
                     auto f = [&](int i) { return __uint_as_float(s[i / 32][i % 32]); };
                     const int key0 = kt * kKeyTile;
-                    const bool edge = key0 < lo_max || key0 + kKeyTile > hi_min;
-                    if (edge) {
+                    if (key0 < lo_max || key0 + kKeyTile > hi_min) {
 #pragma unroll
-                        for (int i = 0; i < kKeyTile; ++i)
-                            if (key0 + i < lo || key0 + i >= hi) s[i / 32][i % 32] = 0xff800000u;
+                        for (int c = 0; c < 4; ++c) {
+                            const int from = lo - key0 - 32 * c, upto = hi - key0 - 32 * c;
+                            if (lo_max > key0 + 32 * c) {
+#pragma unroll
+                                for (int i = 0; i < 32; ++i)
+                                    if (i < from) s[c][i] = 0xff800000u;
+                            }
+                            if (hi_min < key0 + 32 * c + 32) {
+#pragma unroll
+                                for (int i = 0; i < 32; ++i)
+                                    if (i >= upto) s[c][i] = 0xff800000u;
+                            }
+                        }
                     }
                     float t8[8];
 #pragma unroll
@@ -562,7 +570,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             }
             first_run = false;
             if (active) {
-                ok = __all_sync(0xffffffffu, wait_bounded(o_full + 8 * tile, o_ph, wctx, KS_TIMEOUT_TMEM_FULL));
+                ok = __all_sync(0xffffffffu, wait_bounded(o_full + 8 * tile, o_ph, abort_flag, ex.wait_tries, KS_TIMEOUT_TMEM_FULL));
                 if (!ok) break;
                 o_ph ^= 1u;
                 tc_fence_after_sync();
@@ -670,6 +678,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     tc_fence_before_sync();
     __syncthreads();
     if (*abort_flag) {
+        if (threadIdx.x == 0 && a.c.status && *(volatile int *)a.c.status == 0) {
+            *(volatile int *)a.c.status = *abort_flag;
+            __threadfence_system();
+        }
         // a wait ran out: copies and products in flight get time to land before what they target is released
         const unsigned long long t0 = global_timer_ns();
         while (global_timer_ns() - t0 < 200000ull) {
@@ -729,7 +741,7 @@ int launch_attention_chunk(const b200_w8a8_kv_cache *cache, const AttnParams &a,
     static bool attr_set[64][2][2];
     ChunkExtra ex{};
     ex.page_box = cache->page_tokens < kKeyTile ? cache->page_tokens : kKeyTile;
-    ex.wait_limit_ns = wait_limit_ns();
+    ex.wait_tries = (int)std::min(wait_limit_ns() / kWaitNs + 2, 1000000000ull);
     ex.debug_drop_load = take_debug_drop();
     CUtensorMap k, v;
     if (make_page_map(&k, cache->k_pages, cache, ex.page_box) || make_page_map(&v, cache->v_pages, cache, ex.page_box)) return 1;
