@@ -484,12 +484,12 @@ class PagedKVCache:
         _require(k_pages.stride() == v_pages.stride() and k_pages.stride(3) == 1,
                  "k_pages and v_pages have the same strides, the last dimension contiguous")
         _require(k_pages.is_cuda and k_pages.device == v_pages.device, "the pages are on one CUDA device")
-        self.k_pages, self.v_pages, self.dtype, self.device = k_pages, v_pages, k_pages.dtype, k_pages.device
+        self.k_pages, self.v_pages, self.dtype, self.index = k_pages, v_pages, k_pages.dtype, k_pages.get_device()
         pages, heads, page_tokens, d_head = k_pages.shape
         self.n_kv_heads, self.d_head = heads, d_head
         self.struct = _Cache(k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3], _dt(k_pages), pages, page_tokens,
                              heads, d_head)
-        self.ref = ctypes.addressof(self.struct)
+        self.ref = ctypes.byref(self.struct)
 
 
 class PagedBatch:
@@ -505,78 +505,83 @@ class PagedBatch:
         for t in (page_table, q_starts, kv_lens):
             _require(t.dtype == torch.int32 and t.is_contiguous() and t.is_cuda and t.device == kv_lens.device,
                      "page_table, q_starts and kv_lens are contiguous int32 tensors on one CUDA device")
-        self.tensors, self.device = (page_table, q_starts, kv_lens), kv_lens.device
+        self.tensors, self.index = (page_table, q_starts, kv_lens), kv_lens.get_device()
         self.max_new_tokens = max_new_tokens
-        self.struct = _Batch(page_table.data_ptr(), q_starts.data_ptr(), kv_lens.data_ptr(), seqs, page_table.shape[1], 0, 0)
+        self.fields = (page_table.data_ptr(), q_starts.data_ptr(), kv_lens.data_ptr(), seqs, page_table.shape[1])
 
     def of(self, n_tokens):
-        """The struct for row buffers of n_tokens rows, a copy for every call."""
-        st = _Batch.from_buffer_copy(self.struct)
-        st.n_tokens = n_tokens
-        st.max_new_tokens = n_tokens if self.max_new_tokens is None else self.max_new_tokens
-        return st
+        """The struct for row buffers of n_tokens rows, one for every call."""
+        return ctypes.byref(_Batch(*self.fields, n_tokens, n_tokens if self.max_new_tokens is None else self.max_new_tokens))
 
 
-def _same_device(device, *tensors):
-    for t in tensors:
-        _require(t is None or t.device == device, "all tensors of a call are on the cache's device")
+_raw_stream = None  # torch's stream look-up without building a Stream object, where this torch has it
 
 
-def _heads_strides(t, what, heads=None, d_head=None):
-    _require(t.dim() == 3 and t.stride(2) == 1, f"{what} is [tokens, heads, d_head], the last dimension contiguous")
-    _require((heads is None or t.shape[1] == heads) and (d_head is None or t.shape[2] == d_head),
-             f"{what} has shape {tuple(t.shape)}: heads or d_head differ from the cache's")
-    return t.stride(0), t.stride(1)
-
-
-def _call_on(device, fn):
-    """fn(stream) with `device` current, on its current stream."""
+def _call_on(index, fn):
+    """fn(stream) with device `index` current, on its current stream."""
+    global _raw_stream
     import torch
-    if torch.cuda.current_device() == device.index:
-        return fn(torch.cuda.current_stream().cuda_stream)
-    with torch.cuda.device(device):
-        return fn(torch.cuda.current_stream().cuda_stream)
+    if _raw_stream is None:
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda i: torch.cuda.current_stream(i).cuda_stream)
+    if torch.cuda.current_device() == index:
+        return fn(_raw_stream(index))
+    with torch.cuda.device(index):
+        return fn(_raw_stream(index))
+
+
+def _heads_strides(t, what, index, d_head):
+    """Token and head stride of a [tokens, heads, d_head] tensor on device `index`."""
+    if t.dim() != 3 or t.shape[2] != d_head:
+        raise W8A8Error(f"{what} is [tokens, heads, d_head]: got {tuple(t.shape)} for d_head {d_head}")
+    ts, hs, one = t.stride()
+    if one != 1:
+        raise W8A8Error(f"{what}'s last dimension is contiguous")
+    if t.get_device() != index:
+        raise W8A8Error(f"all tensors of a call are on the cache's device: {what} is not")
+    return ts, hs
 
 
 def kv_append(cache, batch, k, v, q=None, q_out=None, norm_eps=None, q_weight=None, k_weight=None, rope_cos=None,
               rope_sin=None, rope_order=None, rope_by_position=False):
     """Writes the new tokens' keys and values to their places in the cache and, with q, the queries to q_out (returned;
     allocated when None), with the RMSNorm of each head (norm_eps not None) and the rotation (rope_order not None) of
-    queries and keys on the way.  k, v, q: [tokens, heads, d_head] of one type (fp32, fp16, bf16), any strides."""
+    queries and keys on the way.  k, v, q: [tokens, heads, d_head] of one type (fp32, fp16, bf16), any strides that are
+    multiples of 16 bytes."""
     import torch
-    x = _New()
-    n, d = k.shape[0], cache.d_head
-    x.k_token_stride, x.k_head_stride = _heads_strides(k, "k", cache.n_kv_heads, d)
-    x.v_token_stride, x.v_head_stride = _heads_strides(v, "v", cache.n_kv_heads, d)
-    _require(v.shape[0] == n and v.dtype == k.dtype, "k and v have the same rows and type")
-    _same_device(cache.device, batch, k, v, q, q_out, q_weight, k_weight, rope_cos, rope_sin)
-    x.k, x.v, x.x_dtype = k.data_ptr(), v.data_ptr(), _dt(k)
-    _require(q is not None or q_out is None, "q_out without q")
+    d, index, n, dtype = cache.d_head, cache.index, k.shape[0], k.dtype
+    kt, kh = _heads_strides(k, "k", index, d)
+    vt, vh = _heads_strides(v, "v", index, d)
+    if k.shape != v.shape or v.dtype != dtype or k.shape[1] != cache.n_kv_heads:
+        raise W8A8Error(f"k and v are [tokens, {cache.n_kv_heads}, {d}] of one type: got {tuple(k.shape)} and {tuple(v.shape)}")
+    if batch.index != index:
+        raise W8A8Error("all tensors of a call are on the cache's device: the batch's are not")
+    qp = qt = qh = op = ot = oh = heads = 0
     if q is not None:
-        x.q_token_stride, x.q_head_stride = _heads_strides(q, "q", None, d)
-        _require(q.shape[0] == n and q.dtype == k.dtype, "q and k have the same rows and type")
+        qt, qh = _heads_strides(q, "q", index, d)
         if q_out is None:
             q_out = torch.empty(q.shape, dtype=cache.dtype, device=q.device)
-        _require(q_out.shape == q.shape and q_out.dtype == cache.dtype, "q_out has q's shape and the cache's type")
-        x.q_out_token_stride, x.q_out_head_stride = _heads_strides(q_out, "q_out")
-        x.q, x.q_out, x.n_heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
-    if norm_eps is not None:
-        x.norm, x.eps = 1, norm_eps
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None:
-            _require(w.dtype == torch.float32 and w.shape == (d,) and w.is_contiguous(), f"{name} is fp32 [d_head]")
-            setattr(x, name, w.data_ptr())
-    if rope_order is not None:
-        x.rope_order = rope_order
-    if x.rope_order:
-        _require(rope_cos is not None and rope_sin is not None, "a rotation needs rope_cos and rope_sin")
+        ot, oh = _heads_strides(q_out, "q_out", index, d)
+        if q.shape[0] != n or q.dtype != dtype or q_out.shape != q.shape or q_out.dtype != cache.dtype:
+            raise W8A8Error("q has k's rows and type, q_out q's shape and the cache's type")
+        qp, op, heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
+    elif q_out is not None:
+        raise W8A8Error("q_out without q")
+    for w in (q_weight, k_weight):
+        if w is not None and (w.dtype != torch.float32 or w.shape != (d,) or not w.is_contiguous() or w.get_device() != index):
+            raise W8A8Error("norm weights are contiguous fp32 [d_head] on the cache's device")
+    cp = sp = rows = 0
+    if rope_order:
+        if rope_cos is None or rope_sin is None:
+            raise W8A8Error("a rotation needs rope_cos and rope_sin")
+        rows = rope_cos.shape[0]
         for t in (rope_cos, rope_sin):
-            _require(t.dtype == torch.float32 and t.dim() == 2 and t.shape[1] == d // 2 and t.is_contiguous()
-                     and t.shape[0] == rope_cos.shape[0], "rope_cos and rope_sin are contiguous fp32 [rows, d_head / 2]")
-        x.rope_cos, x.rope_sin, x.rope_rows = rope_cos.data_ptr(), rope_sin.data_ptr(), rope_cos.shape[0]
-        x.rope_by_position = int(rope_by_position)
-    _check(_call_on(cache.device, lambda st: lib().b200_w8a8_kv_append(cache.ref, ctypes.byref(batch.of(n)), ctypes.byref(x), st)),
-           "kv_append")
+            if t.dtype != torch.float32 or t.shape != (rows, d // 2) or not t.is_contiguous() or t.get_device() != index:
+                raise W8A8Error("rope_cos and rope_sin are contiguous fp32 [rows, d_head / 2] on the cache's device")
+        cp, sp = rope_cos.data_ptr(), rope_sin.data_ptr()
+    x = _New(qp, k.data_ptr(), v.data_ptr(), qt, qh, kt, kh, vt, vh, _dt(k), heads, op, ot, oh, norm_eps is not None,
+             norm_eps or 0.0, _ptr(q_weight), _ptr(k_weight), rope_order or 0, cp, sp, rope_by_position, rows)
+    _check(_call_on(index, lambda st: lib().b200_w8a8_kv_append(cache.ref, batch.of(n), ctypes.byref(x), st)), "kv_append")
     return q_out
 
 
@@ -584,9 +589,9 @@ def make_attention_workspace(cache):
     """Zero-filled scratch for paged_attention over caches of this head size on this device.  Every call leaves its
     counters zero, so one buffer serves all calls that do not overlap on the GPU."""
     import torch
-    with torch.cuda.device(cache.device):
+    with torch.cuda.device(cache.index):
         nbytes = lib().b200_w8a8_paged_attention_workspace_size(cache.d_head)
-        return torch.zeros(nbytes, dtype=torch.uint8, device=cache.device)
+        return torch.zeros(nbytes, dtype=torch.uint8, device=cache.k_pages.device)
 
 
 def paged_attention(q, cache, batch, scale=None, causal_block=1, window=0, out=None, workspace=None):
@@ -594,20 +599,21 @@ def paged_attention(q, cache, batch, scale=None, causal_block=1, window=0, out=N
     causal_block 0: every key; 1: causal; F: causal by blocks of F positions.  window: keys seen, 0 for all.
     scale: 1 / sqrt(d_head) when None.  workspace: from make_attention_workspace (a fresh one when None)."""
     import torch
-    qt, qh = _heads_strides(q, "q", None, cache.d_head)
-    _require(q.dtype == cache.dtype, "q has the cache's type")
+    d, index = cache.d_head, cache.index
+    qt, qh = _heads_strides(q, "q", index, d)
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _require(out.shape == q.shape and out.dtype == q.dtype, "out has q's shape and type")
-    ot, oh = _heads_strides(out, "out")
+    ot, oh = _heads_strides(out, "out", index, d)
+    if q.dtype != cache.dtype or out.dtype != q.dtype or out.shape != q.shape:
+        raise W8A8Error("q has the cache's type, out q's shape and type")
     if workspace is None:
         workspace = make_attention_workspace(cache)
-    _same_device(cache.device, batch, q, out, workspace)
-    if scale is None:
-        scale = cache.d_head ** -0.5
-    _check(_call_on(cache.device, lambda st: lib().b200_w8a8_paged_attention(
-        cache.ref, ctypes.byref(batch.of(q.shape[0])), q.data_ptr(), qt, qh, out.data_ptr(), ot, oh, q.shape[1], scale, causal_block, window,
-        workspace.data_ptr(), workspace.numel() * workspace.element_size(), st)), "paged_attention")
+    if batch.index != index or workspace.get_device() != index:
+        raise W8A8Error("all tensors of a call are on the cache's device: the batch's or the workspace is not")
+    n, heads, _ = q.shape
+    _check(_call_on(index, lambda st: lib().b200_w8a8_paged_attention(
+        cache.ref, batch.of(n), q.data_ptr(), qt, qh, out.data_ptr(), ot, oh, heads, d ** -0.5 if scale is None else scale,
+        causal_block, window, workspace.data_ptr(), workspace.nbytes, st)), "paged_attention")
     return out
 
 

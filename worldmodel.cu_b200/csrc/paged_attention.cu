@@ -357,11 +357,14 @@ int current_device_sms(int &dev) {
 
 }  // namespace
 
-size_t paged_attention_workspace_size(int d_head) {
-    int dev;
-    const int sms = std::min(current_device_sms(dev), kMaxSms);
+static size_t workspace_bytes_for(int d_head, int sms) {
     const size_t rows = 4ull * sms * kRowTile * (d_head + 2) * sizeof(float);
     return kTicketBytes + std::max(rows, attention_chunk_partial_bytes(d_head, sms));
+}
+
+size_t paged_attention_workspace_size(int d_head) {
+    int dev;
+    return workspace_bytes_for(d_head, std::min(current_device_sms(dev), kMaxSms));
 }
 
 int paged_attention(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *batch, const void *q, long long q_ts,
@@ -378,10 +381,11 @@ int paged_attention(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *b
     if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) || ((q_ts | q_hs | o_ts | o_hs) & 7))
         return fail("paged_attention needs 16-byte aligned q and out and strides that are multiples of 8 elements");
     if (((long long)batch->n_tokens * n_heads) >> 30) return fail("paged_attention: n_tokens * n_heads must stay below 2^30");
-    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) ||
-        workspace_bytes < paged_attention_workspace_size(cache->d_head))
+    int dev;
+    const int sms = std::min(current_device_sms(dev), kMaxSms);
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < workspace_bytes_for(cache->d_head, sms))
         return fail("paged_attention needs a 256-byte aligned workspace of %zu bytes, got %zu",
-                    paged_attention_workspace_size(cache->d_head), workspace ? workspace_bytes : (size_t)0);
+                    workspace_bytes_for(cache->d_head, sms), workspace ? workspace_bytes : (size_t)0);
     AttnParams a{};
     a.c = make_view(cache, batch);
     a.q = q; a.q_ts = q_ts; a.q_hs = q_hs;
@@ -395,8 +399,6 @@ int paged_attention(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *b
     a.window = window;
     a.tickets = reinterpret_cast<int *>(workspace);
     a.partials = reinterpret_cast<float *>(reinterpret_cast<char *>(workspace) + kTicketBytes);
-    int dev;
-    const int sms = std::min(current_device_sms(dev), kMaxSms);
     AttnDeviceInfo &di = attn_device_info(dev);
     const bool bf = cache->dtype == B200_DT_BF16;
     // at most so many units of work; the kernels count them in 32 bits
