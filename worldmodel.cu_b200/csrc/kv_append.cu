@@ -5,16 +5,18 @@
 // reference (src/world_cuda.cu:1898-1960) behind wm_cuda_qkv_fused_rms_rope_i32_dequant (src/world_cuda_ops.cu:1229-1305).
 //
 // Every element is read once and written once: memory bound.  A head's d elements are spread over d / 8 lanes, 16 bytes of
-// output each, so the sum of squares and the exchange of pairs that lie half a head apart are shuffles.  A CTA owns a few
-// whole tokens: where they go (sequence, position, page) is found once per token by comparing all sequences' ranges in
-// parallel -- two dependent loads instead of a search per head.
+// output each, so the sum of squares and the exchange of pairs that lie half a head apart are shuffles.  A warp takes whole
+// heads of one token, four at a time in flight, and reads the token's table entries once.  With many tokens a warp has a token
+// to itself; with few, the eight warps of a CTA share one.  Where tokens go (sequence, position, page) is found once per token
+// by comparing all sequences' ranges in parallel: two dependent loads instead of a search per head.
 #include "paged_kv.cuh"
 
 namespace b200 {
 namespace {
 
 constexpr int kAppendThreads = 256;
-constexpr int kMaxTokensPerCta = 16;
+constexpr int kAppendWarps = kAppendThreads / 32;
+constexpr int kInFlight = 4;
 
 struct AppendParams {
     KvView c;
@@ -27,7 +29,7 @@ struct AppendParams {
     float eps;
     const float *q_weight, *k_weight, *cos, *sin;
     int by_position, rope_rows;
-    int tokens_per_cta;
+    int warps_per_token;  // 1 or all of a CTA
 };
 
 struct Place {
@@ -35,41 +37,50 @@ struct Place {
     int rope_row;         // < 0: the token is left out altogether
 };
 
+// Eight elements as they lie in memory, and in fp32.
 template <typename TX>
-__device__ __forceinline__ void load8(const void *base, long long at, float (&x)[8]);
+struct Raw8 {
+    uint4 v;
+    __device__ __forceinline__ void load(const void *base, long long at) {
+        v = *reinterpret_cast<const uint4 *>(reinterpret_cast<const TX *>(base) + at);
+    }
+    __device__ __forceinline__ void unpack(float (&x)[8]) const {
+        float2 f;
+        f = Half2Of<TX>::unpack(v.x); x[0] = f.x; x[1] = f.y;
+        f = Half2Of<TX>::unpack(v.y); x[2] = f.x; x[3] = f.y;
+        f = Half2Of<TX>::unpack(v.z); x[4] = f.x; x[5] = f.y;
+        f = Half2Of<TX>::unpack(v.w); x[6] = f.x; x[7] = f.y;
+    }
+};
 template <>
-__device__ __forceinline__ void load8<float>(const void *base, long long at, float (&x)[8]) {
-    const float4 *p = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(base) + at);
-    const float4 a = p[0], b = p[1];
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
-template <typename T>
-__device__ __forceinline__ void unpack8(const uint4 &r, float (&x)[8]) {
-    float2 f;
-    f = Half2Of<T>::unpack(r.x); x[0] = f.x; x[1] = f.y;
-    f = Half2Of<T>::unpack(r.y); x[2] = f.x; x[3] = f.y;
-    f = Half2Of<T>::unpack(r.z); x[4] = f.x; x[5] = f.y;
-    f = Half2Of<T>::unpack(r.w); x[6] = f.x; x[7] = f.y;
-}
-template <>
-__device__ __forceinline__ void load8<__half>(const void *base, long long at, float (&x)[8]) {
-    unpack8<__half>(*reinterpret_cast<const uint4 *>(reinterpret_cast<const __half *>(base) + at), x);
-}
-template <>
-__device__ __forceinline__ void load8<__nv_bfloat16>(const void *base, long long at, float (&x)[8]) {
-    unpack8<__nv_bfloat16>(*reinterpret_cast<const uint4 *>(reinterpret_cast<const __nv_bfloat16 *>(base) + at), x);
+struct Raw8<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const void *base, long long at) {
+        const float4 *p = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(base) + at);
+        a = p[0];
+        b = p[1];
+    }
+    __device__ __forceinline__ void unpack(float (&x)[8]) const {
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    }
+};
+__device__ __forceinline__ void load4(const float *p, float (&x)[4]) {
+    const float4 v = *reinterpret_cast<const float4 *>(p);
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
 }
 
 template <typename TX, typename TC, int D, int ROPE>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendParams p) {
-    constexpr int L = D / 8;  // lanes per head
-    __shared__ Place place[kMaxTokensPerCta];
+    constexpr int L = D / 8, kHeads = 32 / L;  // lanes per head, heads per warp and pass
+    constexpr int kTable = ROPE == B200_ROPE_HALVES ? 2 : 1;  // vectors of four table entries a lane needs
+    __shared__ Place place[kAppendWarps];
     pdl_trigger();
     pdl_wait();
-    const int t0 = blockIdx.x * p.tokens_per_cta;
-    const int nt = min(p.tokens_per_cta, p.c.n_tokens - t0);
-    if ((int)threadIdx.x < nt) place[threadIdx.x] = {-1, -1};
+    const int warp = threadIdx.x >> 5, per_cta = kAppendWarps / p.warps_per_token;
+    const int t0 = blockIdx.x * per_cta;
+    const int nt = min(per_cta, p.c.n_tokens - t0);
+    if ((int)threadIdx.x < per_cta) place[threadIdx.x] = {-1, -1};
     __syncthreads();
     for (int s = threadIdx.x; s < p.c.n_seqs; s += kAppendThreads) {
         const int q0 = p.c.q_starts[s], q1 = p.c.q_starts[s + 1];
@@ -93,86 +104,88 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendP
     }
     __syncthreads();
 
+    const int local = warp / p.warps_per_token;
+    const Place at = place[local];
+    if (at.kv_offset < 0) return;  // the whole warp
+    const long long t = t0 + local;
+    const int lane = threadIdx.x % L, sub = (threadIdx.x & 31) / L;
     const int heads = p.n_heads + 2 * p.c.n_kv_heads;
-    const int units = nt * heads;
-    const int lane = threadIdx.x % L;
-    // every warp runs whole iterations, so the shuffles below have all their lanes
-    constexpr int kUnitsPerWarp = 32 / L, kUnitsPerCta = kAppendThreads / L;
-    for (int base = (threadIdx.x / 32) * kUnitsPerWarp; base < units; base += kUnitsPerCta) {
-        const int unit = base + (threadIdx.x % 32) / L;
-        const int tok = min(unit / heads, nt - 1), head = unit % heads;
-        const Place at = place[tok];
-        const bool live = unit < units && at.kv_offset >= 0;
-        const long long t = t0 + tok;
-        const bool is_q = head < p.n_heads, is_v = head >= p.n_heads + p.c.n_kv_heads;
-        const int h = is_q ? head : is_v ? head - p.n_heads - p.c.n_kv_heads : head - p.n_heads;
-        float x[8] = {};
-        if (live) {
-            if (is_q) load8<TX>(p.q, t * p.q_ts + h * p.q_hs + lane * 8, x);
-            else if (is_v) load8<TX>(p.v, t * p.v_ts + h * p.v_hs + lane * 8, x);
-            else load8<TX>(p.k, t * p.k_ts + h * p.k_hs + lane * 8, x);
+    float cs[kTable][4], sn[kTable][4];
+    if (ROPE != B200_ROPE_NONE) {
+        const long long row = (long long)at.rope_row * (D / 2) + (ROPE == B200_ROPE_HALVES ? (lane % (L / 2)) * 8 : lane * 4);
+#pragma unroll
+        for (int g = 0; g < kTable; ++g) {
+            load4(p.cos + row + 4 * g, cs[g]);
+            load4(p.sin + row + 4 * g, sn[g]);
         }
-        if (p.norm) {
-            float ss = 0.0f;
+    }
+    for (int base = (warp % p.warps_per_token) * kHeads; base < heads; base += kInFlight * p.warps_per_token * kHeads) {
+        Raw8<TX> raw[kInFlight];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
+        for (int u = 0; u < kInFlight; ++u) {
+            const int head = min(base + u * p.warps_per_token * kHeads + sub, heads - 1);
+            const bool is_q = head < p.n_heads, is_v = head >= p.n_heads + p.c.n_kv_heads;
+            const int h = is_q ? head : is_v ? head - p.n_heads - p.c.n_kv_heads : head - p.n_heads;
+            const void *src = is_q ? p.q : is_v ? p.v : p.k;
+            raw[u].load(src, t * (is_q ? p.q_ts : is_v ? p.v_ts : p.k_ts) + h * (is_q ? p.q_hs : is_v ? p.v_hs : p.k_hs) + lane * 8);
+        }
 #pragma unroll
-            for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            if (!is_v) {
-                const float inv = rsqrtf(ss * (1.0f / D) + p.eps);
+        for (int u = 0; u < kInFlight; ++u) {
+            if (base + u * p.warps_per_token * kHeads >= heads) break;  // warp-uniform
+            const int head = base + u * p.warps_per_token * kHeads + sub;
+            const bool live = head < heads, is_q = head < p.n_heads, is_v = head >= p.n_heads + p.c.n_kv_heads;
+            const int h = is_q ? head : is_v ? head - p.n_heads - p.c.n_kv_heads : head - p.n_heads;
+            float x[8];
+            raw[u].unpack(x);
+            if (p.norm) {
+                float ss = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
+#pragma unroll
+                for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                const float inv = is_v ? 1.0f : rsqrtf(ss * (1.0f / D) + p.eps);
                 const float *w = is_q ? p.q_weight : p.k_weight;
-                if (w) {
-                    const float4 a = *reinterpret_cast<const float4 *>(w + lane * 8);
-                    const float4 b = *reinterpret_cast<const float4 *>(w + lane * 8 + 4);
-                    x[0] *= a.x; x[1] *= a.y; x[2] *= a.z; x[3] *= a.w;
-                    x[4] *= b.x; x[5] *= b.y; x[6] *= b.z; x[7] *= b.w;
+                if (w && !is_v) {
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        float ww[4];
+                        load4(w + lane * 8 + 4 * g, ww);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) x[4 * g + j] *= ww[j];
+                    }
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] *= inv;
             }
-        }
-        TC *dst;
-        if (is_q) dst = reinterpret_cast<TC *>(p.q_out) + t * p.qo_ts + h * p.qo_hs;
-        else dst = reinterpret_cast<TC *>(is_v ? p.c.v : p.c.k) + at.kv_offset + h * p.c.head_stride;
-        if (ROPE == B200_ROPE_HALVES) {
-            float y[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = __shfl_xor_sync(0xffffffffu, x[j], L / 2);
-            if (live && !is_v) {
-                const long long row = (long long)at.rope_row * (D / 2) + (lane % (L / 2)) * 8;
+            if (ROPE == B200_ROPE_HALVES) {
                 const float sign = lane < L / 2 ? -1.0f : 1.0f;
 #pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    const float4 c = *reinterpret_cast<const float4 *>(p.cos + row + 4 * g);
-                    const float4 s = *reinterpret_cast<const float4 *>(p.sin + row + 4 * g);
-                    x[4 * g + 0] = fmaf(sign * y[4 * g + 0], s.x, x[4 * g + 0] * c.x);
-                    x[4 * g + 1] = fmaf(sign * y[4 * g + 1], s.y, x[4 * g + 1] * c.y);
-                    x[4 * g + 2] = fmaf(sign * y[4 * g + 2], s.z, x[4 * g + 2] * c.z);
-                    x[4 * g + 3] = fmaf(sign * y[4 * g + 3], s.w, x[4 * g + 3] * c.w);
+                for (int j = 0; j < 8; ++j) {
+                    const float y = sign * __shfl_xor_sync(0xffffffffu, x[j], L / 2);
+                    if (!is_v) x[j] = fmaf(y, sn[j / 4][j % 4], x[j] * cs[j / 4][j % 4]);
+                }
+            } else if (ROPE != B200_ROPE_NONE && !is_v) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float a = x[2 * j], b = x[2 * j + 1];
+                    x[2 * j] = fmaf(-b, sn[0][j], a * cs[0][j]);
+                    x[2 * j + 1] = fmaf(a, sn[0][j], b * cs[0][j]);
                 }
             }
-        } else if (ROPE != B200_ROPE_NONE && live && !is_v) {
-            const long long row = (long long)at.rope_row * (D / 2) + lane * 4;
-            const float4 c = *reinterpret_cast<const float4 *>(p.cos + row);
-            const float4 s = *reinterpret_cast<const float4 *>(p.sin + row);
-            const float cc[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float a = x[2 * j], b = x[2 * j + 1];
-                x[2 * j] = fmaf(-b, sn[j], a * cc[j]);
-                x[2 * j + 1] = fmaf(a, sn[j], b * cc[j]);
+            if (!live) continue;
+            TC *dst;
+            if (is_q) dst = reinterpret_cast<TC *>(p.q_out) + t * p.qo_ts + h * p.qo_hs;
+            else dst = reinterpret_cast<TC *>(is_v ? p.c.v : p.c.k) + at.kv_offset + h * p.c.head_stride;
+            if (ROPE == B200_ROPE_SPLIT && !is_v) {
+                *reinterpret_cast<uint2 *>(dst + lane * 4) =
+                    make_uint2(Half2Of<TC>::pack(x[0], x[2]), Half2Of<TC>::pack(x[4], x[6]));
+                *reinterpret_cast<uint2 *>(dst + D / 2 + lane * 4) =
+                    make_uint2(Half2Of<TC>::pack(x[1], x[3]), Half2Of<TC>::pack(x[5], x[7]));
+            } else {
+                *reinterpret_cast<uint4 *>(dst + lane * 8) =
+                    make_uint4(Half2Of<TC>::pack(x[0], x[1]), Half2Of<TC>::pack(x[2], x[3]), Half2Of<TC>::pack(x[4], x[5]),
+                               Half2Of<TC>::pack(x[6], x[7]));
             }
-        }
-        if (!live) continue;
-        if (ROPE == B200_ROPE_SPLIT && !is_v) {
-            *reinterpret_cast<uint2 *>(dst + lane * 4) =
-                make_uint2(Half2Of<TC>::pack(x[0], x[2]), Half2Of<TC>::pack(x[4], x[6]));
-            *reinterpret_cast<uint2 *>(dst + D / 2 + lane * 4) =
-                make_uint2(Half2Of<TC>::pack(x[1], x[3]), Half2Of<TC>::pack(x[5], x[7]));
-        } else {
-            *reinterpret_cast<uint4 *>(dst + lane * 8) =
-                make_uint4(Half2Of<TC>::pack(x[0], x[1]), Half2Of<TC>::pack(x[2], x[3]), Half2Of<TC>::pack(x[4], x[5]),
-                           Half2Of<TC>::pack(x[6], x[7]));
         }
     }
 }
@@ -232,8 +245,9 @@ int kv_append(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *batch, 
     p.n_heads = x->q ? x->n_heads : 0;
     p.norm = x->norm != 0; p.eps = x->eps; p.q_weight = x->q_weight; p.k_weight = x->k_weight;
     p.cos = x->rope_cos; p.sin = x->rope_sin; p.by_position = x->rope_by_position != 0; p.rope_rows = x->rope_rows;
-    p.tokens_per_cta = 1;
-    const unsigned grid = (unsigned)((batch->n_tokens + p.tokens_per_cta - 1) / p.tokens_per_cta);
+    p.warps_per_token = batch->n_tokens >= 4096 ? 1 : kAppendWarps;
+    const int per_cta = kAppendWarps / p.warps_per_token;
+    const unsigned grid = (unsigned)((batch->n_tokens + per_cta - 1) / per_cta);
     if (cache->dtype == B200_DT_F16) {
         if (cache->d_head == 64) launch_append<__half, 64>(p, x->x_dtype, x->rope_order, dim3(grid), stream);
         else launch_append<__half, 128>(p, x->x_dtype, x->rope_order, dim3(grid), stream);
