@@ -6,7 +6,7 @@
 //
 // Every element is read once and written once: memory bound.  A head's d elements are spread over d / 8 lanes, 16 bytes of
 // output each, so the sum of squares and the exchange of pairs that lie half a head apart are shuffles.  A warp takes whole
-// heads of one token, four at a time in flight, and reads the token's table entries once.  With many tokens a warp has a token
+// heads of one token, several at a time in flight, and reads the token's table entries once.  With many tokens a warp has a token
 // to itself; with few, the eight warps of a CTA share one.  Where tokens go (sequence, position, page) is found once per token
 // by comparing all sequences' ranges in parallel: two dependent loads instead of a search per head.
 #include "paged_kv.cuh"
@@ -16,14 +16,15 @@ namespace {
 
 constexpr int kAppendThreads = 256;
 constexpr int kAppendWarps = kAppendThreads / 32;
-constexpr int kInFlight = 4;
 
 struct AppendParams {
     KvView c;
     const void *q, *k, *v;
-    long long q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
+    long long q_ts, k_ts, v_ts;
+    int q_hs, k_hs, v_hs;
     void *q_out;
-    long long qo_ts, qo_hs;
+    long long qo_ts;
+    int qo_hs, c_hs;  // c_hs: the cache's head stride
     int n_heads;  // of q; 0 without q
     int norm;
     float eps;
@@ -41,45 +42,59 @@ struct Place {
 template <typename TX>
 struct Raw8 {
     uint4 v;
-    __device__ __forceinline__ void load(const void *base, long long at) {
-        v = *reinterpret_cast<const uint4 *>(reinterpret_cast<const TX *>(base) + at);
+    __device__ __forceinline__ void load(const TX *p) {
+        v = *reinterpret_cast<const uint4 *>(p);
     }
-    __device__ __forceinline__ void unpack(float (&x)[8]) const {
+    __device__ __forceinline__ void unpack(uint64_t (&x)[4]) const {
         float2 f;
-        f = Half2Of<TX>::unpack(v.x); x[0] = f.x; x[1] = f.y;
-        f = Half2Of<TX>::unpack(v.y); x[2] = f.x; x[3] = f.y;
-        f = Half2Of<TX>::unpack(v.z); x[4] = f.x; x[5] = f.y;
-        f = Half2Of<TX>::unpack(v.w); x[6] = f.x; x[7] = f.y;
+        f = Half2Of<TX>::unpack(v.x); x[0] = pair2(f.x, f.y);
+        f = Half2Of<TX>::unpack(v.y); x[1] = pair2(f.x, f.y);
+        f = Half2Of<TX>::unpack(v.z); x[2] = pair2(f.x, f.y);
+        f = Half2Of<TX>::unpack(v.w); x[3] = pair2(f.x, f.y);
     }
 };
 template <>
 struct Raw8<float> {
     float4 a, b;
-    __device__ __forceinline__ void load(const void *base, long long at) {
-        const float4 *p = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(base) + at);
-        a = p[0];
-        b = p[1];
+    __device__ __forceinline__ void load(const float *p) {
+        a = *reinterpret_cast<const float4 *>(p);
+        b = *reinterpret_cast<const float4 *>(p + 4);
     }
-    __device__ __forceinline__ void unpack(float (&x)[8]) const {
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    __device__ __forceinline__ void unpack(uint64_t (&x)[4]) const {
+        x[0] = pair2(a.x, a.y); x[1] = pair2(a.z, a.w);
+        x[2] = pair2(b.x, b.y); x[3] = pair2(b.z, b.w);
     }
 };
-__device__ __forceinline__ void load4(const float *p, float (&x)[4]) {
-    const float4 v = *reinterpret_cast<const float4 *>(p);
-    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-}
-
 template <typename TX, typename TC, int D, int ROPE>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(const AppendParams p) {
+    constexpr int kInFlight = sizeof(TX) == 4 ? 2 : 4;  // 32 bytes of fp32 a lane, 16 of others: 64 bytes on the way
     constexpr int L = D / 8, kHeads = 32 / L;  // lanes per head, heads per warp and pass
-    constexpr int kTable = ROPE == B200_ROPE_HALVES ? 2 : 1;  // vectors of four table entries a lane needs
     __shared__ Place place[kAppendWarps];
     pdl_trigger();
     pdl_wait();
     const int warp = threadIdx.x >> 5, per_cta = kAppendWarps / p.warps_per_token;
     const int t0 = blockIdx.x * per_cta;
     const int nt = min(per_cta, p.c.n_tokens - t0);
+    // a warp's own part of the rows, the first of it on the way while the token's place is looked up
+    const int local = warp / p.warps_per_token;
+    const int lane = threadIdx.x % L, sub = (threadIdx.x & 31) / L;
+    const int first_v = p.n_heads + p.c.n_kv_heads, heads = first_v + p.c.n_kv_heads;
+    const int step = p.warps_per_token * kHeads, start = (warp % p.warps_per_token) * kHeads;
+    const long long t = min(t0 + local, p.c.n_tokens - 1);
+    Raw8<TX> raw[kInFlight];
+    const TX *q_row = reinterpret_cast<const TX *>(p.q) + t * p.q_ts + lane * 8;
+    const TX *k_row = reinterpret_cast<const TX *>(p.k) + t * p.k_ts + lane * 8;
+    const TX *v_row = reinterpret_cast<const TX *>(p.v) + t * p.v_ts + lane * 8;
+    auto fetch = [&](int base) {
+#pragma unroll
+        for (int u = 0; u < kInFlight; ++u) {
+            const int head = min(base + u * step + sub, heads - 1);
+            if (head < p.n_heads) raw[u].load(q_row + (long long)head * p.q_hs);
+            else if (head < first_v) raw[u].load(k_row + (long long)(head - p.n_heads) * p.k_hs);
+            else raw[u].load(v_row + (long long)(head - first_v) * p.v_hs);
+        }
+    };
+    fetch(start);
     if ((int)threadIdx.x < per_cta) place[threadIdx.x] = {-1, -1};
     __syncthreads();
     for (int s = threadIdx.x; s < p.c.n_seqs; s += kAppendThreads) {
@@ -104,87 +119,89 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendP
     }
     __syncthreads();
 
-    const int local = warp / p.warps_per_token;
     const Place at = place[local];
     if (at.kv_offset < 0) return;  // the whole warp
-    const long long t = t0 + local;
-    const int lane = threadIdx.x % L, sub = (threadIdx.x & 31) / L;
-    const int heads = p.n_heads + 2 * p.c.n_kv_heads;
-    float cs[kTable][4], sn[kTable][4];
-    if (ROPE != B200_ROPE_NONE) {
-        const long long row = (long long)at.rope_row * (D / 2) + (ROPE == B200_ROPE_HALVES ? (lane % (L / 2)) * 8 : lane * 4);
+    // Of the pairs that this lane turns: HALVES, two vectors of (x, y) pairs of neighbours; else four pairs (a, b), of which
+    // (c, c) and (-s, s) are kept
+    uint64_t cs[4], sn[4];
+    if (ROPE == B200_ROPE_HALVES) {
+        const float sign = lane < L / 2 ? -1.0f : 1.0f;
+        const long long row = (long long)at.rope_row * (D / 2) + (lane % (L / 2)) * 8;
 #pragma unroll
-        for (int g = 0; g < kTable; ++g) {
-            load4(p.cos + row + 4 * g, cs[g]);
-            load4(p.sin + row + 4 * g, sn[g]);
+        for (int g = 0; g < 2; ++g) {
+            const float4 c = *reinterpret_cast<const float4 *>(p.cos + row + 4 * g);
+            const float4 s = *reinterpret_cast<const float4 *>(p.sin + row + 4 * g);
+            cs[2 * g] = pair2(c.x, c.y); cs[2 * g + 1] = pair2(c.z, c.w);
+            sn[2 * g] = pair2(sign * s.x, sign * s.y); sn[2 * g + 1] = pair2(sign * s.z, sign * s.w);
         }
+    } else if (ROPE != B200_ROPE_NONE) {
+        const long long row = (long long)at.rope_row * (D / 2) + lane * 4;
+        const float4 c = *reinterpret_cast<const float4 *>(p.cos + row), s = *reinterpret_cast<const float4 *>(p.sin + row);
+        cs[0] = pair2(c.x, c.x); cs[1] = pair2(c.y, c.y); cs[2] = pair2(c.z, c.z); cs[3] = pair2(c.w, c.w);
+        sn[0] = pair2(-s.x, s.x); sn[1] = pair2(-s.y, s.y); sn[2] = pair2(-s.z, s.z); sn[3] = pair2(-s.w, s.w);
     }
-    for (int base = (warp % p.warps_per_token) * kHeads; base < heads; base += kInFlight * p.warps_per_token * kHeads) {
-        Raw8<TX> raw[kInFlight];
+    TC *const q_dst = reinterpret_cast<TC *>(p.q_out) + t * p.qo_ts;
+    TC *const k_dst = reinterpret_cast<TC *>(p.c.k) + at.kv_offset, *const v_dst = reinterpret_cast<TC *>(p.c.v) + at.kv_offset;
+    for (int base = start; base < heads; base += kInFlight * step) {
+        if (base != start) fetch(base);
 #pragma unroll
         for (int u = 0; u < kInFlight; ++u) {
-            const int head = min(base + u * p.warps_per_token * kHeads + sub, heads - 1);
-            const bool is_q = head < p.n_heads, is_v = head >= p.n_heads + p.c.n_kv_heads;
-            const int h = is_q ? head : is_v ? head - p.n_heads - p.c.n_kv_heads : head - p.n_heads;
-            const void *src = is_q ? p.q : is_v ? p.v : p.k;
-            raw[u].load(src, t * (is_q ? p.q_ts : is_v ? p.v_ts : p.k_ts) + h * (is_q ? p.q_hs : is_v ? p.v_hs : p.k_hs) + lane * 8);
-        }
-#pragma unroll
-        for (int u = 0; u < kInFlight; ++u) {
-            if (base + u * p.warps_per_token * kHeads >= heads) break;  // warp-uniform
-            const int head = base + u * p.warps_per_token * kHeads + sub;
-            const bool live = head < heads, is_q = head < p.n_heads, is_v = head >= p.n_heads + p.c.n_kv_heads;
-            const int h = is_q ? head : is_v ? head - p.n_heads - p.c.n_kv_heads : head - p.n_heads;
-            float x[8];
+            if (base + u * step >= heads) break;  // warp-uniform
+            const int head = base + u * step + sub;
+            const bool live = head < heads, is_q = head < p.n_heads, is_v = head >= first_v;
+            uint64_t x[4];
             raw[u].unpack(x);
             if (p.norm) {
-                float ss = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
+                const uint64_t sq = add2(fma2(x[0], x[0], mul2(x[1], x[1])), fma2(x[2], x[2], mul2(x[3], x[3])));
+                float ss, more;
+                unpair2(sq, ss, more);
+                ss += more;
 #pragma unroll
                 for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
                 const float inv = is_v ? 1.0f : rsqrtf(ss * (1.0f / D) + p.eps);
+                const uint64_t inv2 = pair2(inv, inv);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = mul2(x[j], inv2);
                 const float *w = is_q ? p.q_weight : p.k_weight;
                 if (w && !is_v) {
 #pragma unroll
                     for (int g = 0; g < 2; ++g) {
-                        float ww[4];
-                        load4(w + lane * 8 + 4 * g, ww);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) x[4 * g + j] *= ww[j];
+                        const float4 ww = *reinterpret_cast<const float4 *>(w + lane * 8 + 4 * g);
+                        x[2 * g] = mul2(x[2 * g], pair2(ww.x, ww.y));
+                        x[2 * g + 1] = mul2(x[2 * g + 1], pair2(ww.z, ww.w));
                     }
                 }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] *= inv;
             }
             if (ROPE == B200_ROPE_HALVES) {
-                const float sign = lane < L / 2 ? -1.0f : 1.0f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float y = sign * __shfl_xor_sync(0xffffffffu, x[j], L / 2);
-                    if (!is_v) x[j] = fmaf(y, sn[j / 4][j % 4], x[j] * cs[j / 4][j % 4]);
+                for (int j = 0; j < 4; ++j) {
+                    const uint64_t y = __shfl_xor_sync(0xffffffffu, (unsigned long long)x[j], L / 2);
+                    if (!is_v) x[j] = fma2(y, sn[j], mul2(x[j], cs[j]));
                 }
             } else if (ROPE != B200_ROPE_NONE && !is_v) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float a = x[2 * j], b = x[2 * j + 1];
-                    x[2 * j] = fmaf(-b, sn[0][j], a * cs[0][j]);
-                    x[2 * j + 1] = fmaf(a, sn[0][j], b * cs[0][j]);
+                    float a, b;
+                    unpair2(x[j], a, b);
+                    x[j] = fma2(pair2(b, a), sn[j], mul2(x[j], cs[j]));
                 }
             }
             if (!live) continue;
             TC *dst;
-            if (is_q) dst = reinterpret_cast<TC *>(p.q_out) + t * p.qo_ts + h * p.qo_hs;
-            else dst = reinterpret_cast<TC *>(is_v ? p.c.v : p.c.k) + at.kv_offset + h * p.c.head_stride;
+            if (is_q) dst = q_dst + (long long)head * p.qo_hs;
+            else if (!is_v) dst = k_dst + (long long)(head - p.n_heads) * p.c_hs;
+            else dst = v_dst + (long long)(head - first_v) * p.c_hs;
+            float a[4], b[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) unpair2(x[j], a[j], b[j]);
             if (ROPE == B200_ROPE_SPLIT && !is_v) {
-                *reinterpret_cast<uint2 *>(dst + lane * 4) =
-                    make_uint2(Half2Of<TC>::pack(x[0], x[2]), Half2Of<TC>::pack(x[4], x[6]));
+                *reinterpret_cast<uint2 *>(dst + lane * 4) = make_uint2(Half2Of<TC>::pack(a[0], a[1]), Half2Of<TC>::pack(a[2], a[3]));
                 *reinterpret_cast<uint2 *>(dst + D / 2 + lane * 4) =
-                    make_uint2(Half2Of<TC>::pack(x[1], x[3]), Half2Of<TC>::pack(x[5], x[7]));
+                    make_uint2(Half2Of<TC>::pack(b[0], b[1]), Half2Of<TC>::pack(b[2], b[3]));
             } else {
                 *reinterpret_cast<uint4 *>(dst + lane * 8) =
-                    make_uint4(Half2Of<TC>::pack(x[0], x[1]), Half2Of<TC>::pack(x[2], x[3]), Half2Of<TC>::pack(x[4], x[5]),
-                               Half2Of<TC>::pack(x[6], x[7]));
+                    make_uint4(Half2Of<TC>::pack(a[0], b[0]), Half2Of<TC>::pack(a[1], b[1]), Half2Of<TC>::pack(a[2], b[2]),
+                               Half2Of<TC>::pack(a[3], b[3]));
             }
         }
     }
@@ -236,12 +253,16 @@ int kv_append(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *batch, 
                                (x->q ? x->q_token_stride | x->q_head_stride : 0);
     if ((in_strides & (unit - 1)) || (x->q && ((x->q_out_token_stride | x->q_out_head_stride) & 7)))
         return fail("kv_append needs strides that are multiples of 16 bytes");
+    const int64_t head_strides[] = {x->k_head_stride, x->v_head_stride, cache->head_stride, x->q ? x->q_head_stride : 0,
+                                    x->q ? x->q_out_head_stride : 0};
+    for (int64_t h : head_strides)
+        if (h < 0 || h >> 31) return fail("kv_append needs head strides from 0 to 2^31 - 1 elements, got %lld", (long long)h);
     AppendParams p{};
     p.c = make_view(cache, batch);
     p.q = x->q; p.k = x->k; p.v = x->v;
-    p.q_ts = x->q_token_stride; p.q_hs = x->q_head_stride; p.k_ts = x->k_token_stride; p.k_hs = x->k_head_stride;
-    p.v_ts = x->v_token_stride; p.v_hs = x->v_head_stride;
-    p.q_out = x->q_out; p.qo_ts = x->q_out_token_stride; p.qo_hs = x->q_out_head_stride;
+    p.q_ts = x->q_token_stride; p.q_hs = (int)x->q_head_stride; p.k_ts = x->k_token_stride; p.k_hs = (int)x->k_head_stride;
+    p.v_ts = x->v_token_stride; p.v_hs = (int)x->v_head_stride;
+    p.q_out = x->q_out; p.qo_ts = x->q_out_token_stride; p.qo_hs = (int)x->q_out_head_stride; p.c_hs = (int)cache->head_stride;
     p.n_heads = x->q ? x->n_heads : 0;
     p.norm = x->norm != 0; p.eps = x->eps; p.q_weight = x->q_weight; p.k_weight = x->k_weight;
     p.cos = x->rope_cos; p.sin = x->rope_sin; p.by_position = x->rope_by_position != 0; p.rope_rows = x->rope_rows;

@@ -113,25 +113,6 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void *map, uint6
         : "memory");
 }
 
-// two fp32 values per instruction
-__device__ __forceinline__ uint64_t pair2(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void unpair2(uint64_t v, float &a, float &b) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 // 2^x for x in [-inf, 2^22) on the multiply-add pipe: x = n + f, n the nearest integer, |f| <= 1/2; 2^f by the polynomial of
 // least relative error over that interval among those that are exact at 0 (degree 3: 1.0e-4, for weights rounded to bf16 by
 // up to 2^-9; degree 4: 2.8e-6, for fp16's 2^-12), n added to the exponent.  x <= -127, -inf too, gives exactly 0.
