@@ -286,29 +286,55 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attention_rows_kernel(const A
             }
             __syncthreads();
             if (last_flag) {
-                for (int i = threadIdx.x; i < rows * (D / 2); i += kRowsThreads) {
-                    const int r = i / (D / 2), col = 2 * (i % (D / 2));
+                // join: all maxima and sums to shared memory, a warp per row turns them into factors, then a thread sums four
+                // columns of a row over the parts, several of which are on the way at a time
+                __threadfence();
+                const int parts = final - first + 1;
+                float *factor = reinterpret_cast<float *>(smem), *part_sum = factor + parts * kRowTile;
+                auto part_of = [&](int c) {
+                    return a.partials + (long long)(2 * (first + c) + (c == 0 ? 1 : 0)) * C::kPartialFloats;
+                };
+                for (int i = threadIdx.x; i < parts * rows; i += kRowsThreads) {
+                    const int c = i / rows, r = i % rows;
+                    factor[c * kRowTile + r] = __ldcg(part_of(c) + kRowTile * D + r);
+                    part_sum[c * kRowTile + r] = __ldcg(part_of(c) + kRowTile * D + kRowTile + r);
+                }
+                __syncthreads();
+                for (int r = warp; r < rows; r += kRowsThreads / 32) {
                     float top = -INFINITY, sum = 0.0f;
-                    float2 v = make_float2(0.0f, 0.0f);
-                    for (int c = first; c <= final; ++c) {
-                        const float *pc = a.partials + (long long)(2 * c + (c == first ? 1 : 0)) * C::kPartialFloats;
-                        const float pm = __ldcg(pc + kRowTile * D + r), ps = __ldcg(pc + kRowTile * D + kRowTile + r);
-                        const float2 u = __ldcg(reinterpret_cast<const float2 *>(pc + r * D + col));
-                        if (pm == -INFINITY) continue;
-                        const float mn = fmaxf(top, pm);
-                        const float fa = top == -INFINITY ? 0.0f : exp2f((top - mn) * a.scale_log2);
-                        const float fb = exp2f((pm - mn) * a.scale_log2);
-                        sum = sum * fa + ps * fb;
-                        v.x = v.x * fa + u.x * fb;
-                        v.y = v.y * fa + u.y * fb;
-                        top = mn;
+                    for (int c = lane; c < parts; c += 32) top = fmaxf(top, factor[c * kRowTile + r]);
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    const float ref = top == -INFINITY ? 0.0f : top;
+                    for (int c = lane; c < parts; c += 32) {
+                        const float f = exp2f((factor[c * kRowTile + r] - ref) * a.scale_log2);
+                        factor[c * kRowTile + r] = f;
+                        sum = fmaf(part_sum[c * kRowTile + r], f, sum);
                     }
-                    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    if (lane == 0) warp_sum[0][r] = sum > 0.0f ? 1.0f / sum : 0.0f;
+                }
+                __syncthreads();
+                for (int i = threadIdx.x; i < rows * (D / 4); i += kRowsThreads) {
+                    const int r = i / (D / 4), col = 4 * (i % (D / 4));
+                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+                    for (int c = 0; c < parts; ++c) {
+                        const float4 u = __ldcg(reinterpret_cast<const float4 *>(part_of(c) + r * D + col));
+                        const float f = factor[c * kRowTile + r];
+                        v.x = fmaf(u.x, f, v.x);
+                        v.y = fmaf(u.y, f, v.y);
+                        v.z = fmaf(u.z, f, v.z);
+                        v.w = fmaf(u.w, f, v.w);
+                    }
+                    const float inv = warp_sum[0][r];
                     const int rr = r0 + r;
                     const int tok = a.by_group.div(rr);
                     T *dst = reinterpret_cast<T *>(a.out) + (long long)(it.seq.q0 + tok) * a.o_ts +
                              (long long)(it.h * a.group + rr - tok * a.group) * a.o_hs + col;
-                    *reinterpret_cast<uint32_t *>(dst) = Half2Of<T>::pack(v.x * inv, v.y * inv);
+                    *reinterpret_cast<uint2 *>(dst) =
+                        make_uint2(Half2Of<T>::pack(v.x * inv, v.y * inv), Half2Of<T>::pack(v.z * inv, v.w * inv));
                 }
             }
         }
