@@ -498,6 +498,18 @@ int b200_w8a8_layer_qkv(void *ctx, const b200_w8a8_layer *layer, const float *to
 int b200_w8a8_layer_after_attention(void *ctx, const b200_w8a8_layer *layer, const float *attn, const float *tokens,
                                     float *tokens_next, int n_tokens, void *stream);
 
+/* The same layer as ONE call, its attention included: norm, QKV linear, per-head RMSNorm + rotation (B200_ROPE_SPLIT; tables
+ * as b200_w8a8_kv_append reads them, rope_rows rows by token or by position), append to the paged cache, attention of the new
+ * tokens over it (scale 1 / sqrt(d_head), mask as in b200_w8a8_paged_attention), and everything behind it;
+ * queries, keys, values and the attention's output are of the cache's 16-bit type.  batch->n_tokens rows of tokens and
+ * tokens_next (which may be one buffer), every row a token of some sequence; n_heads, n_kv_heads and d_head (64 or 128) are
+ * the context's.  workspace: as in b200_w8a8_paged_attention.  What the reference does from src/world_cuda.cu:1819 to :2330
+ * with its own ring and attention. */
+int b200_w8a8_layer_forward_paged(void *ctx, const b200_w8a8_layer *layer, const b200_w8a8_kv_cache *cache,
+                                  const b200_w8a8_kv_batch *batch, const float *tokens, const float *rope_cos,
+                                  const float *rope_sin, int rope_by_position, int rope_rows, float *tokens_next,
+                                  int causal_block, int window, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- offline packed-weight file (HOST side; the writer needs no GPU) ---------------- */
 
 /* Writes the int8 codes (slab layout) and per-channel scales of every layer, plus the three

@@ -319,3 +319,32 @@ def test_pages_and_lengths_outside_the_cache_are_reported_once(pkg):
                 call([0, 1], 3, what)
                 torch.cuda.synchronize()
                 assert pkg.poll_status() == 0
+
+
+def test_a_wait_that_runs_out_is_reported_once(pkg):
+    """One page load left out by the test switch: the kernel gives up after 5 ms, drains and returns; the next call says so
+    once; with the workspace zeroed again everything is as before."""
+    L = pkg.lib()
+    seqs, heads, kv, d = [(300, 2000), (40, 64)], 4, 2, 128
+    g = torch.Generator().manual_seed(1)
+    k_pages, v_pages, table, _ = pr.make_cache(seqs, 32, kv, d, torch.float16, "heads", g, DEV)
+    cache = pkg.PagedKVCache(k_pages, v_pages)
+    batch = pkg.PagedBatch(table, pr.starts_of(seqs, DEV), pr.lens_of(seqs, DEV))
+    q = torch.randn(340, heads, d, generator=g).half().to(DEV)
+    ws = pkg.make_attention_workspace(cache)
+    want = pkg.paged_attention(q, cache, batch, workspace=ws)
+    torch.cuda.synchronize()
+    try:
+        L.b200_w8a8_debug_set_wait_limit_ns(5_000_000)
+        L.b200_w8a8_debug_drop_operand_load(1)
+        pkg.paged_attention(q, cache, batch, workspace=ws)
+        torch.cuda.synchronize()
+        with pytest.raises(pkg.W8A8Error, match="gave up a bounded wait"):
+            pkg.paged_attention(q, cache, batch, workspace=ws)
+    finally:
+        L.b200_w8a8_debug_drop_operand_load(0)
+        L.b200_w8a8_debug_set_wait_limit_ns(0)
+    ws.zero_()
+    assert torch.equal(pkg.paged_attention(q, cache, batch, workspace=ws), want)
+    torch.cuda.synchronize()
+    assert pkg.poll_status() == 0

@@ -99,6 +99,8 @@ _PROTOTYPES = {
     "b200_w8a8_layer_ctx_device_bytes": (c_size_t, [c_void_p]),
     "b200_w8a8_layer_qkv": (c_int, [c_void_p] * 8 + [c_int, c_void_p]),
     "b200_w8a8_layer_after_attention": (c_int, [c_void_p] * 5 + [c_int, c_void_p]),
+    "b200_w8a8_layer_forward_paged": (c_int, [c_void_p] * 7 + [c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_size_t,
+                                                               c_void_p]),
     "b200_w8a8_weight_file_create": (c_void_p, [ctypes.c_char_p, c_int, c_int, c_int, c_int]),
     "b200_w8a8_weight_file_add_layer": (c_int, [c_void_p] + [c_void_p] * 8 + [c_int]),
     "b200_w8a8_weight_file_close": (c_int, [c_void_p]),
@@ -660,6 +662,28 @@ class ReferenceLayerDriver:
         st = layer if isinstance(layer, _Layer) else self.pack(layer)
         _check(lib().b200_w8a8_layer_after_attention(self.handle, ctypes.byref(st), _ptr(attn), _ptr(tokens), _ptr(out),
                                                      tokens.shape[0], _stream()), "layer_after_attention")
+        return out
+
+    def forward_paged(self, layer, tokens, rope_cos, rope_sin, cache, batch, causal_block=1, window=0, out=None,
+                      workspace=None, rope_by_position=False):
+        """The whole layer with its attention over the paged cache (b200_w8a8_layer_forward_paged): appends the new tokens'
+        keys and values to `cache` and returns the next token stream [tokens, d_model]."""
+        import torch
+        d = self.dims[0]
+        out = torch.empty_like(tokens) if out is None else out
+        workspace = make_attention_workspace(cache) if workspace is None else workspace
+        rows = rope_cos.shape[0]
+        for t, shape in ((tokens, (tokens.shape[0], d)), (out, tokens.shape), (rope_cos, (rows, cache.d_head // 2)),
+                         (rope_sin, (rows, cache.d_head // 2))):
+            if t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous() or t.get_device() != cache.index:
+                raise W8A8Error("tokens, out and the tables are contiguous fp32 tensors on the cache's device")
+        if batch.index != cache.index or workspace.get_device() != cache.index:
+            raise W8A8Error("all tensors of a call are on the cache's device: the batch's or the workspace is not")
+        st = layer if isinstance(layer, _Layer) else self.pack(layer)
+        _check(_call_on(cache.index, lambda stream: lib().b200_w8a8_layer_forward_paged(
+            self.handle, ctypes.byref(st), cache.ref, batch.of(tokens.shape[0]), _ptr(tokens), _ptr(rope_cos), _ptr(rope_sin),
+            int(rope_by_position), rows, _ptr(out), causal_block, window, workspace.data_ptr(), workspace.nbytes, stream)),
+            "layer_forward_paged")
         return out
 
     def close(self):
