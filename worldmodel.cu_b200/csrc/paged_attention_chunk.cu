@@ -31,7 +31,8 @@ template <int D>
 struct ChunkCfg {
     static constexpr int kTileBytes = D / 64 * kSlabBytes;
     static constexpr int kStages = D == 128 ? 5 : 8;
-    static constexpr int kSmemBytes = (2 + kStages) * kTileBytes + 1024 + 256;
+    static constexpr int kBars = 2 * kStages + 18;
+    static constexpr int kSmemBytes = (2 + kStages) * kTileBytes + kBars * 8 + 16 + 1024;  // and alignment
     static constexpr int kWarpPartial = 32 * (D + 2);  // floats: 32 rows x D, maxima, sums
 };
 
@@ -210,6 +211,9 @@ struct ChunkExtra {
     int debug_drop_load;
 };
 
+// An item of one row tile: both accumulators work on it, KV tiles in turn, and are joined at the end of a run.
+__device__ __forceinline__ bool is_shared(const Item &it) { return it.rows - it.rt * kChunkRows <= 128; }
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kChunkThreads, 1)
     attention_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -222,18 +226,19 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     uint8_t *ring = smem + 2 * C::kTileBytes;
     // barriers: [stage] pages have landed; [stage] their products are done; [row tile] its queries are in shared memory; its
     // scores are in tensor memory; [row tile][half] half of its weights are there and O is rescaled; [row tile] the last product
-    // of a run has landed
+    // of a run has landed; [warp] where both work on one row tile: B's maxima and sums are known, and A has taken B's part over
     uint64_t *bars = reinterpret_cast<uint64_t *>(ring + C::kStages * C::kTileBytes);
     const uint32_t kv_full = smem_u32(bars), kv_empty = kv_full + 8 * C::kStages, q_ready = kv_empty + 8 * C::kStages;
     const uint32_t s_full = q_ready + 16, p_ready = s_full + 16, o_full = p_ready + 32;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * C::kStages + 10);
+    const uint32_t b_known = o_full + 16, b_taken = b_known + 32;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + C::kBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     pdl_trigger();
     if (threadIdx.x == 0) {
         // four arrivals, one per softmax warp, where such a warp signals; one everywhere else
-        for (int i = 0; i < 2 * C::kStages + 10; ++i) {
+        for (int i = 0; i < C::kBars; ++i) {
             const int j = i - 2 * C::kStages;
             mbar_init(bars + i, j == 0 || j == 1 || (j >= 4 && j < 8) ? 4 : 1);
         }
@@ -322,8 +327,64 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 uint32_t ph = 0, q_ph = 0, p_ph = 0;  // q_ph, p_ph: bit x is the parity of row tile x's barriers
                 while (now.kt0 < now.kt1) {
                     const int kt0 = now.kt0, kt1 = now.kt1;
-                    const int tiles = it.rows - it.rt * kChunkRows > 128 ? 2 : 1;
                     bool ok = true;
+                    if (is_shared(it)) {
+                        // one row tile, whose queries serve both accumulators: A takes the run's KV tiles 0, 2, ..., B 1, 3, ...
+                        const int n = kt1 - kt0;
+                        auto ahead = [&](int by, uint32_t &bar, uint32_t &par) {  // stage `by` behind s, its barrier and parity
+                            int st = s + by;
+                            par = ph;
+                            if (st >= C::kStages) { st -= C::kStages; par ^= 1u; }
+                            bar = kv_full + 8 * st;
+                            return st;
+                        };
+                        ok = wait_bounded(q_ready, q_ph & 1u, abort_flag, ex.wait_tries, KS_TIMEOUT_SOFTMAX);
+                        q_ph ^= 1u;
+                        tc_fence_after_sync();
+#pragma unroll 1
+                        for (int i = -2; ok && i < n; ++i) {
+                            const int r = i & 1;
+                            uint32_t bar, par;
+                            if (i >= 0) {
+                                const int vs = ahead(1, bar, par);
+                                ok = wait_bounded(bar, par, abort_flag, ex.wait_tries, KS_TIMEOUT_SMEM_FULL);
+                                const uint64_t vd = v_desc + (uint64_t)(vs * (C::kTileBytes >> 4));
+#pragma unroll 1
+                                for (int half = 0; ok && half < 2; ++half) {
+                                    ok = wait_bounded(p_ready + 16 * r + 8 * half, (p_ph >> r) & 1u, abort_flag, ex.wait_tries,
+                                                      KS_TIMEOUT_SOFTMAX);
+                                    if (!ok) break;
+                                    tc_fence_after_sync();
+                                    umma_f16_ts4(tmem_o + r * D, tmem + r * kKeyTile + 32 * half,
+                                                 vd + (uint64_t)(half * (64 * 128 >> 4)), idesc_o, i >= 2 || half);
+                                }
+                                if (!ok) break;
+                                p_ph ^= 1u << r;
+                                if (i + 2 >= n) commit_to(o_full + 8 * r);
+                                commit_to(kv_empty + 8 * vs);
+                            }
+                            if (i + 2 < n) {  // K of tile i + 2: its stage is two for each tile ahead of tile max(i, 0)'s
+                                const int ks = ahead(2 * (i + 2 - (i > 0 ? i : 0)), bar, par);
+                                ok = wait_bounded(bar, par, abort_flag, ex.wait_tries, KS_TIMEOUT_SMEM_FULL);
+                                if (!ok) break;
+                                tc_fence_after_sync();
+                                const uint64_t kd = k_desc + (uint64_t)(ks * (C::kTileBytes >> 4));
+#pragma unroll
+                                for (int d = 0; d < D / 64; ++d)
+                                    umma_f16_ss4(tmem + r * kKeyTile, q_desc + (uint64_t)(d * (kSlabBytes >> 4)),
+                                                 kd + (uint64_t)(d * (kSlabBytes >> 4)), idesc_s, d != 0);
+                                commit_to(s_full + 8 * r);
+                                commit_to(kv_empty + 8 * ks);
+                            }
+                            if (i >= 0) {
+                                s += 2;
+                                if (s >= C::kStages) { s -= C::kStages; ph ^= 1u; }
+                            }
+                        }
+                        if (!ok) break;
+                        walk.advance<kChunkRows, kKeyTile, kChunkExtra>(a);
+                        continue;
+                    }
                     for (int kt = kt0 - 1; kt < kt1; ++kt) {
                         // V of tile kt and K of tile kt + 1 are the next two stages of the ring
                         const int vs = s;
@@ -338,7 +399,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                         }
                         if (!ok) break;
 #pragma unroll 1
-                        for (int r = 0; r < tiles; ++r) {
+                        for (int r = 0; r < 2; ++r) {
                             if (kt >= kt0) {
                                 const uint64_t vd = v_desc + (uint64_t)(vs * (C::kTileBytes >> 4));
                                 const uint32_t par = (p_ph >> r) & 1u;
@@ -413,46 +474,47 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             __syncwarp();
             if (lane == 0) arrive_on(q_ready + 8 * tile);
         };
-        uint32_t s_ph = 0, o_ph = 0;
-        int v_stage = 1, v_ph = 0;  // of the ring, and its parity: where the values of the current tile arrive
+        uint32_t s_ph = 0, o_ph = 0, b_ph = 0, known_ph = 0;  // b_ph: of B's o_full, as A sees it
+        const float *b_stats = reinterpret_cast<const float *>(smem + C::kTileBytes + sub * 32 * 128);  // in B's idle queries
+        int tiles_before = 0;  // KV tiles of this CTA before the current run: where in the ring its values arrive
         bool ok = true, first_run = true;
         while (now.kt0 < now.kt1) {
             const int kt0 = now.kt0, kt1 = now.kt1;
-            const int row0 = it.rt * kChunkRows + tile * 128 + sub * 32;
-            const bool active = it.rt * kChunkRows + tile * 128 < it.rows;
+            const bool shared = is_shared(it);
+            const int row0 = it.rt * kChunkRows + (shared ? 0 : tile * 128) + sub * 32;
+            const bool active = shared || it.rt * kChunkRows + tile * 128 < it.rows;
+            const int kt_first = shared ? kt0 + tile : kt0, kt_step = shared ? 2 : 1;
             float m = -INFINITY, l = 0.0f;
             const int item_lo = it.lo, item_hi = it.hi;
             if (active) {
-                if (first_run) load_q(row0);
+                if (first_run && (tile == 0 || !shared)) load_q(row0);
                 int lo = 0, hi = 0x7fffffff;  // a row that is not there masks nothing
                 if (row0 + lane < it.rows)
                     visible_keys(a, it.seq.keys - it.seq.n + a.by_group.div(row0 + lane), it.seq.keys, lo, hi);
                 const int lo_max = __reduce_max_sync(0xffffffffu, lo), hi_min = __reduce_min_sync(0xffffffffu, hi);
-                for (int kt = kt0; kt < kt1; ++kt) {
+                for (int kt = kt_first; kt < kt1; kt += kt_step) {
                     ok = __all_sync(0xffffffffu, wait_bounded(s_full + 8 * tile, s_ph, abort_flag, ex.wait_tries, KS_TIMEOUT_SOFTMAX));
                     if (!ok) break;
                     s_ph ^= 1u;
                     tc_fence_after_sync();
-                    if (tile == 0) {
-                        // Values of keys that the item's rows do not see may be anything, NaN too, and 0 x NaN is no zero: the
-                        // four warps of tile A clear them before their weights let the products of this tile begin
-                        if (kt * kKeyTile < item_lo || (kt + 1) * kKeyTile > item_hi) {
-                            ok = __all_sync(0xffffffffu, wait_bounded(kv_full + 8 * v_stage, v_ph, abort_flag, ex.wait_tries, KS_TIMEOUT_SMEM_FULL));
-                            if (!ok) break;
-                            uint8_t *v = ring + v_stage * C::kTileBytes;
-                            for (int row = sub * 32 + lane / 8; row < sub * 32 + 32; row += 4) {
-                                const int key = kt * kKeyTile + row;
-                                if (key < item_lo || key >= item_hi) {
+                    // Values of keys that the item's rows do not see may be anything, NaN too, and 0 x NaN is no zero: the four
+                    // warps whose product comes first clear them before their weights let it begin
+                    if ((tile == 0 || shared) && (kt * kKeyTile < item_lo || (kt + 1) * kKeyTile > item_hi)) {
+                        const unsigned at = 2u * (unsigned)(tiles_before + kt - kt0) + 1u, stage = at % C::kStages;
+                        ok = __all_sync(0xffffffffu, wait_bounded(kv_full + 8 * stage, at / C::kStages & 1u, abort_flag,
+                                                                  ex.wait_tries, KS_TIMEOUT_SMEM_FULL));
+                        if (!ok) break;
+                        uint8_t *v = ring + stage * C::kTileBytes;
+                        for (int row = sub * 32 + lane / 8; row < sub * 32 + 32; row += 4) {
+                            const int key = kt * kKeyTile + row;
+                            if (key < item_lo || key >= item_hi) {
 #pragma unroll
-                                    for (int d = 0; d < D / 64; ++d)
-                                        *reinterpret_cast<uint4 *>(v + d * kSlabBytes + row * 128 + (lane & 7) * 16) =
-                                            make_uint4(0, 0, 0, 0);
-                                }
+                                for (int d = 0; d < D / 64; ++d)
+                                    *reinterpret_cast<uint4 *>(v + d * kSlabBytes + row * 128 + (lane & 7) * 16) =
+                                        make_uint4(0, 0, 0, 0);
                             }
-                            fence_proxy_async_smem();
                         }
-                        v_stage += 2;
-                        if (v_stage >= C::kStages) { v_stage -= C::kStages; v_ph ^= 1; }
+                        fence_proxy_async_smem();
                     }
                     uint32_t s[4][32];
 #pragma unroll
@@ -485,7 +547,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                         t8[i] = fmaxf(t8[i], f(i + kKeyTile - 8));
                     }
                     const float top = max3(max3(t8[0], t8[1], t8[2]), max3(t8[3], t8[4], t8[5]), fmaxf(t8[6], t8[7]));
-                    if (kt == kt0) {
+                    if (kt == kt_first) {
                         m = top;
                     } else if (__any_sync(0xffffffffu, (top - m) * a.scale_log2 > kLazyRescale)) {
                         const float mn = fmaxf(m, top);
@@ -539,9 +601,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 if (!ok) break;
             }
             // what the end of this run needs, then on to the next item, whose queries come to L2 meanwhile
+            tiles_before += kt1 - kt0;
             const int first = now.first, final = now.final, rows = it.rows, head0 = it.h * a.group, q0 = it.seq.q0;
             advance();
-            const bool more = now.kt0 < now.kt1 && it.rt * kChunkRows + tile * 128 < it.rows;
+            const bool more = now.kt0 < now.kt1 && it.rt * kChunkRows + tile * 128 < it.rows;  // queries to fetch
             {
                 const int r = it.rt * kChunkRows + tile * 128 + sub * 32 + lane;
                 if (more && r < it.rows) {
@@ -551,41 +614,97 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             }
             first_run = false;
             if (active) {
+                const bool mine_any = kt_first < kt1;  // B has nothing in a run of one KV tile
+                if (shared && tile == 1) {
+                    float *stats = const_cast<float *>(b_stats);
+                    stats[lane] = m;
+                    stats[32 + lane] = l;
+                    __syncwarp();
+                    if (lane == 0) arrive_on(b_known + 8 * sub);
+                    ok = __all_sync(0xffffffffu, wait_bounded(b_taken + 8 * sub, known_ph, abort_flag, ex.wait_tries, KS_TIMEOUT_TMEM_FULL));
+                    if (!ok) break;
+                    known_ph ^= 1u;
+                    if (mine_any) o_ph ^= 1u;
+                    if (more) load_q(it.rt * kChunkRows + tile * 128 + sub * 32);
+                    continue;
+                }
                 ok = __all_sync(0xffffffffu, wait_bounded(o_full + 8 * tile, o_ph, abort_flag, ex.wait_tries, KS_TIMEOUT_TMEM_FULL));
                 if (!ok) break;
                 o_ph ^= 1u;
+                // this row's factors of the two accumulators
+                float fa = 1.0f, fb = 0.0f;
+                if (shared) {
+                    const bool b_any = kt0 + 1 < kt1;
+                    ok = wait_bounded(b_known + 8 * sub, known_ph, abort_flag, ex.wait_tries, KS_TIMEOUT_TMEM_FULL);
+                    if (ok && b_any) ok = wait_bounded(o_full + 8, b_ph, abort_flag, ex.wait_tries, KS_TIMEOUT_TMEM_FULL);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    known_ph ^= 1u;
+                    if (b_any) {
+                        b_ph ^= 1u;
+                        const float mb = b_stats[lane], lb = b_stats[32 + lane], top = fmaxf(m, mb);
+                        const float ref = top == -INFINITY ? 0.0f : top;
+                        fa = fast_ex2((m - ref) * a.scale_log2);
+                        fb = fast_ex2((mb - ref) * a.scale_log2);
+                        m = top;
+                        l = l * fa + lb * fb;
+                    }
+                } else {
+                    b_ph ^= 1u;
+                }
+                const bool two = shared && kt0 + 1 < kt1;
+                auto b_done = [&]() {  // B may go on to its next run
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) arrive_on(b_taken + 8 * sub);
+                };
+                auto load_o = [&](int c, float (&o)[32]) {  // columns 32 c .. of this row's sum
+                    uint32_t u[32];
+                    tmem_ld_32x32(to + 32 * c, u);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(u[i]);
+                    if (two) {
+                        tmem_ld_32x32(to + D + 32 * c, u);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = fmaf(__uint_as_float(u[i]), fb, o[i] * fa);
+                    }
+                };
                 tc_fence_after_sync();
                 bool write = first == final;
                 float inv = l > 0.0f ? 1.0f / l : 0.0f;
                 if (write) {
 #pragma unroll
                     for (int c = 0; c < D / 32; ++c) {
-                        uint32_t o[32];
-                        tmem_ld_32x32(to + 32 * c, o);
-                        tmem_ld_wait();
-                        auto g = [&](int i) { return __uint_as_float(o[i]) * inv; };
+                        float o[32];
+                        load_o(c, o);
+                        auto g = [&](int i) { return o[i] * inv; };
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             *reinterpret_cast<uint4 *>(chunk_at(lane, 4 * c + i)) =
                                 make_uint4(Half2Of<T>::pack(g(8 * i), g(8 * i + 1)), Half2Of<T>::pack(g(8 * i + 2), g(8 * i + 3)),
                                            Half2Of<T>::pack(g(8 * i + 4), g(8 * i + 5)), Half2Of<T>::pack(g(8 * i + 6), g(8 * i + 7)));
                     }
+                    if (shared) b_done();
                 } else {
                     // [slot of the CTA][warp]: columns in vectors of four, 32 rows each
-                    auto part_of = [&](int cta) {
+                    const int parts = final - first + 1;
+                    auto slot_of = [&](int cta) {
                         return a.partials + ((long long)(2 * cta + (cta == first ? 1 : 0)) * 8 + warp) * C::kWarpPartial;
                     };
-                    float *part = part_of((int)blockIdx.x);
+                    auto part_of = [&](int i) { return slot_of(first + i); };
+                    float *part = slot_of((int)blockIdx.x);
 #pragma unroll
                     for (int c = 0; c < D / 32; ++c) {
-                        uint32_t o[32];
-                        tmem_ld_32x32(to + 32 * c, o);
-                        tmem_ld_wait();
+                        float o[32];
+                        load_o(c, o);
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
-                            *reinterpret_cast<uint4 *>(part + ((8 * c + i) * 32 + lane) * 4) =
-                                make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                            *reinterpret_cast<float4 *>(part + ((8 * c + i) * 32 + lane) * 4) =
+                                make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                     }
+                    if (shared) b_done();
                     part[32 * D + lane] = m;
                     part[32 * D + 32 + lane] = l;
                     __threadfence();
@@ -594,36 +713,38 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     if (lane == 0) {
                         int *ticket = a.tickets + first * 8 + warp;
                         before = atomicAdd(ticket, 1);
-                        if (before == final - first) *ticket = 0;  // zero again for the next launch
+                        if (before == parts - 1) *ticket = 0;  // zero again for the next launch
                     }
                     before = __shfl_sync(0xffffffffu, before, 0);
                     __threadfence();
-                    write = before == final - first;
-                    if (write) {  // the last of the item's CTAs joins the parts, in the order of their keys
+                    write = before == parts - 1;
+                    if (write) {  // the last of the item's warps for these rows joins the parts, in the order of their keys
                         float top = -INFINITY, sum = 0.0f;
-                        for (int cta = first; cta <= final; ++cta) top = fmaxf(top, __ldcg(part_of(cta) + 32 * D + lane));
+#pragma unroll 8
+                        for (int i = 0; i < parts; ++i) top = fmaxf(top, __ldcg(part_of(i) + 32 * D + lane));
                         const float ref = top == -INFINITY ? 0.0f : top;
-                        for (int cta = first; cta <= final; ++cta) {
-                            const float *pc = part_of(cta) + 32 * D + lane;
+#pragma unroll 4
+                        for (int i = 0; i < parts; ++i) {
+                            const float *pc = part_of(i) + 32 * D + lane;
                             sum = fmaf(__ldcg(pc + 32), fast_ex2((__ldcg(pc) - ref) * a.scale_log2), sum);
                         }
                         inv = sum > 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll 1
                         for (int c = 0; c < D / 32; ++c) {
                             float v[32] = {};
-#pragma unroll 1
-                            for (int cta = first; cta <= final; ++cta) {
-                                const float *pc = part_of(cta);
+#pragma unroll 2
+                            for (int i = 0; i < parts; ++i) {
+                                const float *pc = part_of(i);
                                 const float g = fast_ex2((__ldcg(pc + 32 * D + lane) - ref) * a.scale_log2);
                                 float4 u[8];
 #pragma unroll
-                                for (int i = 0; i < 8; ++i) u[i] = __ldcg(reinterpret_cast<const float4 *>(pc) + (8 * c + i) * 32 + lane);
+                                for (int j = 0; j < 8; ++j) u[j] = __ldcg(reinterpret_cast<const float4 *>(pc) + (8 * c + j) * 32 + lane);
 #pragma unroll
-                                for (int i = 0; i < 8; ++i) {
-                                    v[4 * i] = fmaf(u[i].x, g, v[4 * i]);
-                                    v[4 * i + 1] = fmaf(u[i].y, g, v[4 * i + 1]);
-                                    v[4 * i + 2] = fmaf(u[i].z, g, v[4 * i + 2]);
-                                    v[4 * i + 3] = fmaf(u[i].w, g, v[4 * i + 3]);
+                                for (int j = 0; j < 8; ++j) {
+                                    v[4 * j] = fmaf(u[j].x, g, v[4 * j]);
+                                    v[4 * j + 1] = fmaf(u[j].y, g, v[4 * j + 1]);
+                                    v[4 * j + 2] = fmaf(u[j].z, g, v[4 * j + 2]);
+                                    v[4 * j + 3] = fmaf(u[j].w, g, v[4 * j + 3]);
                                 }
                             }
 #pragma unroll
