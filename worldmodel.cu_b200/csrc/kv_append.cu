@@ -7,8 +7,8 @@
 // Every element is read once and written once: memory bound.  A head's d elements are spread over d / 8 lanes, 16 bytes of
 // output each, so the sum of squares and the exchange of pairs that lie half a head apart are shuffles.  A warp takes whole
 // heads of one token, several at a time in flight, and reads the token's table entries once.  With many tokens a warp has a token
-// to itself; with few, the eight warps of a CTA share one.  Where tokens go (sequence, position, page) is found once per token
-// by comparing all sequences' ranges in parallel: two dependent loads instead of a search per head.
+// to itself; with few, the eight warps of a CTA share one.  Each warp finds its token's place by itself, while its first heads
+// are on the way: 32 probes at a time into the sequences' starts, then length and page; no barrier.
 #include "paged_kv.cuh"
 
 namespace b200 {
@@ -33,10 +33,19 @@ struct AppendParams {
     int warps_per_token;  // 1 or all of a CTA
 };
 
-struct Place {
-    long long kv_offset;  // element offset of (page, 0, slot), < 0: not appended
-    int rope_row;         // < 0: the token is left out altogether
-};
+// The sequence whose new tokens hold row t, -1 if none does: the warp probes 32 starts at a time.
+__device__ __forceinline__ int last_start(const KvView &c, int t) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = c.n_seqs + 1;  // among q_starts[lo .. hi - 1]
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, i = lo + lane * step;
+        const int found = __popc(__ballot_sync(0xffffffffu, i < hi && c.q_starts[min(i, c.n_seqs)] <= t));
+        if (found == 0) return -1;
+        lo += (found - 1) * step;
+        hi = min(hi, lo + step);
+    }
+    return lo < c.n_seqs && c.q_starts[lo] <= t && t < c.q_starts[lo + 1] ? lo : -1;
+}
 
 // Eight elements as they lie in memory, and in fp32.
 template <typename TX>
@@ -69,12 +78,10 @@ template <typename TX, typename TC, int D, int ROPE>
 __global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(const AppendParams p) {
     constexpr int kInFlight = sizeof(TX) == 4 ? 2 : 4;  // 32 bytes of fp32 a lane, 16 of others: 64 bytes on the way
     constexpr int L = D / 8, kHeads = 32 / L;  // lanes per head, heads per warp and pass
-    __shared__ Place place[kAppendWarps];
     pdl_trigger();
     pdl_wait();
     const int warp = threadIdx.x >> 5, per_cta = kAppendWarps / p.warps_per_token;
     const int t0 = blockIdx.x * per_cta;
-    const int nt = min(per_cta, p.c.n_tokens - t0);
     // a warp's own part of the rows, the first of it on the way while the token's place is looked up
     const int local = warp / p.warps_per_token;
     const int lane = threadIdx.x % L, sub = (threadIdx.x & 31) / L;
@@ -95,38 +102,26 @@ __global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(const Appe
         }
     };
     fetch(start);
-    if ((int)threadIdx.x < per_cta) place[threadIdx.x] = {-1, -1};
-    __syncthreads();
-    for (int s = threadIdx.x; s < p.c.n_seqs; s += kAppendThreads) {
-        const int q0 = p.c.q_starts[s], q1 = p.c.q_starts[s + 1];
-        const int first = max(q0, t0), last = min(q1, t0 + nt);
-        for (int t = first; t < last; ++t) {
-            const int pos = p.c.kv_lens[s] - (q1 - t);
-            if (pos < 0) continue;
-            const int index = pos >> p.c.page_shift;
-            int page = -1;
-            if (index < p.c.max_pages) page = p.c.page_table[(long long)s * p.c.max_pages + index];
-            Place at;
-            at.rope_row = p.by_position ? pos : t;
-            at.kv_offset = -1;
-            if (page < 0 || page >= p.c.n_pages || (ROPE != B200_ROPE_NONE && at.rope_row >= p.rope_rows)) {
-                report_bad_page(p.c);
-                continue;
-            }
-            at.kv_offset = page * p.c.page_stride + (pos & ((1 << p.c.page_shift) - 1)) * p.c.token_stride;
-            place[t - t0] = at;
-        }
+    if (t0 + local >= p.c.n_tokens) return;  // the whole warp, here and below
+    // where the token goes: its sequence is the last one that starts at or before it
+    const int seq = last_start(p.c, (int)t);
+    if (seq < 0) return;
+    const int pos = p.c.kv_lens[seq] - (p.c.q_starts[seq + 1] - (int)t);
+    if (pos < 0) return;
+    const int index = pos >> p.c.page_shift, rope_row = p.by_position ? pos : (int)t;
+    const int page = index < p.c.max_pages ? p.c.page_table[(long long)seq * p.c.max_pages + index] : -1;
+    if (page < 0 || page >= p.c.n_pages || (ROPE != B200_ROPE_NONE && rope_row >= p.rope_rows)) {
+        report_bad_page(p.c);
+        return;
     }
-    __syncthreads();
-
-    const Place at = place[local];
-    if (at.kv_offset < 0) return;  // the whole warp
+    const long long kv_offset =
+        page * p.c.page_stride + (pos & ((1 << p.c.page_shift) - 1)) * p.c.token_stride;
     // Of the pairs that this lane turns: HALVES, two vectors of (x, y) pairs of neighbours; else four pairs (a, b), of which
     // (c, c) and (-s, s) are kept
     uint64_t cs[4], sn[4];
     if (ROPE == B200_ROPE_HALVES) {
         const float sign = lane < L / 2 ? -1.0f : 1.0f;
-        const long long row = (long long)at.rope_row * (D / 2) + (lane % (L / 2)) * 8;
+        const long long row = (long long)rope_row * (D / 2) + (lane % (L / 2)) * 8;
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
             const float4 c = *reinterpret_cast<const float4 *>(p.cos + row + 4 * g);
@@ -135,13 +130,13 @@ __global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(const Appe
             sn[2 * g] = pair2(sign * s.x, sign * s.y); sn[2 * g + 1] = pair2(sign * s.z, sign * s.w);
         }
     } else if (ROPE != B200_ROPE_NONE) {
-        const long long row = (long long)at.rope_row * (D / 2) + lane * 4;
+        const long long row = (long long)rope_row * (D / 2) + lane * 4;
         const float4 c = *reinterpret_cast<const float4 *>(p.cos + row), s = *reinterpret_cast<const float4 *>(p.sin + row);
         cs[0] = pair2(c.x, c.x); cs[1] = pair2(c.y, c.y); cs[2] = pair2(c.z, c.z); cs[3] = pair2(c.w, c.w);
         sn[0] = pair2(-s.x, s.x); sn[1] = pair2(-s.y, s.y); sn[2] = pair2(-s.z, s.z); sn[3] = pair2(-s.w, s.w);
     }
     TC *const q_dst = reinterpret_cast<TC *>(p.q_out) + t * p.qo_ts;
-    TC *const k_dst = reinterpret_cast<TC *>(p.c.k) + at.kv_offset, *const v_dst = reinterpret_cast<TC *>(p.c.v) + at.kv_offset;
+    TC *const k_dst = reinterpret_cast<TC *>(p.c.k) + kv_offset, *const v_dst = reinterpret_cast<TC *>(p.c.v) + kv_offset;
     for (int base = start; base < heads; base += kInFlight * step) {
         if (base != start) fetch(base);
 #pragma unroll
