@@ -11,6 +11,8 @@
 // last contributor, found by a ticket, joins them in order of their keys, so results do not depend on timing.
 #pragma once
 
+#include <mutex>
+
 #include "paged_kv.cuh"
 
 namespace b200 {
@@ -48,8 +50,20 @@ int launch_attention_chunk(const b200_w8a8_kv_cache *cache, const AttnParams &a,
 
 namespace {
 
-constexpr int kTicketBytes = 16384;           // counters at the start of the workspace: one per warp that joins
-constexpr int kMaxSms = kTicketBytes / 4 / 8;  // eight such warps per SM
+constexpr int kTicketBytes = 32768;                // counters at the start of the workspace
+constexpr int kMaxSms = kTicketBytes / 4 / (8 * 3);  // the chunk kernel's joining warps have three each
+
+// Raises a kernel's dynamic shared-memory limit on the current device once; the flag is only touched under the mutex.
+template <typename Kernel>
+int raise_smem_limit(bool &done, Kernel kernel, int bytes, const char *what) {
+    static std::mutex mu;
+    std::lock_guard<std::mutex> hold(mu);
+    if (done) return 0;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return fail("cudaFuncSetAttribute(%s, smem=%d): %s", what, bytes, cudaGetErrorString(e));
+    done = true;
+    return 0;
+}
 
 // Cuts `total` units into `runs` runs of equal length, the first `rest` of them one unit longer.
 struct RunMap {

@@ -2,12 +2,22 @@
 //
 // A work item is 256 query rows of one (sequence, key head), as two tiles A and B of 128 rows.  Per KV tile and row tile
 //     S = Q K^T (tensor memory, fp32)  ->  P = 2^(c (S - m)) (16 bits, over S in tensor memory)  ->  O += P V.
-// One warp fetches pages by TMA into a ring of K and V tiles, one issues the products, and four each own the softmax of
-// A and of B, one thread per row, so that row maxima and sums need no exchange.  While A's weights are computed the tensor
-// core works on B.  The running maximum moves only when a row has outgrown it by 2^8 (weights stay below 2^8, exact in the
-// quotient), so O in tensor memory is rescaled rarely.
+// One warp fetches pages by TMA into a ring of K and V tiles, one thread issues the products, and four warps each own the
+// softmax of A and of B, one thread per row, so that row maxima and sums need no exchange.  While A's weights are computed the
+// tensor core works on B.  The running maximum moves only when a row has outgrown it by 2^8 (weights stay below 2^8, and the
+// factor cancels in the quotient), so O in tensor memory is rescaled rarely.  Weights are rounded to the cache's type, half a
+// step each: that is what the tensor core takes; their sum is taken before, in fp32.
 // Keys stay K-major as they lie in the page, values are read in the same layout as the MN-major operand: nothing is
 // transposed.  Rows of V outside the sequence are zeroed in shared memory before their product, since 0 x NaN is no zero.
+// An item of at most 128 rows has no second row tile: both accumulators work on it, KV tiles in turn.
+//
+// Measured: a prompt of 8192 tokens (32 / 8 heads of 128, bf16, causal) 470 us = 1.17 PFLOP/s, 71 % of the rate of a large
+// library product; a frame of 512 tokens over 8704 keys (32 / 16 heads of 64, fp16) 63 us.  The tensor pipe is busy 56 % of the
+// cycles, the special-function unit 43 %, the issue slots 43 %: what bounds the loop is the chain scores -> maximum -> weights
+// -> product of a row tile (about 3400 cycles a KV tile, of which the products are 1000), of which two run against each other.
+// Tried and slower: half a row per thread with sixteen softmax warps (563 us), KV tiles in halves with two score buffers (517),
+// a thread per row tile to issue products (583 when their batches mix, 501 when the softmax warps take turns), all
+// exponentials on the special-function unit (476), rolled loops over 32 scores (529).
 #include <cuda.h>
 
 #include <algorithm>
@@ -23,9 +33,12 @@ constexpr int kChunkThreads = 384;  // three warpgroups; warps 10 and 11 only fi
 constexpr int kSoftmaxRegs = 224, kOtherRegs = 56;
 constexpr int kChunkRows = 256;   // two row tiles
 constexpr int kKeyTile = 128;
+// measured 1 / 2 / 3 / 5 / 8: the prompt 659 / 532 / 469 / 474 / 487 us (its first CTA has 50 items of one to four tiles), 80 rows
+// of 16 sequences 33.5 / 31.6 / 30.6 / 29.3 / 28.9 us, the frame 64.5 / 64.0 / 62.9 / 64.1 / 65.5 us
 constexpr int kChunkExtra = 3;
 constexpr int kSlabBytes = 128 * 128;  // 128 rows of 64 16-bit elements, 128-byte swizzle
 constexpr float kLazyRescale = 8.0f;   // log2 of how far a weight may exceed one
+constexpr int kJoinAtOnce = 8;         // parts of an item that are joined in one step
 
 template <int D>
 struct ChunkCfg {
@@ -673,8 +686,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 };
                 tc_fence_after_sync();
                 bool write = first == final;
-                float inv = l > 0.0f ? 1.0f / l : 0.0f;
                 if (write) {
+                    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
                     for (int c = 0; c < D / 32; ++c) {
                         float o[32];
@@ -693,7 +706,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     auto slot_of = [&](int cta) {
                         return a.partials + ((long long)(2 * cta + (cta == first ? 1 : 0)) * 8 + warp) * C::kWarpPartial;
                     };
-                    auto part_of = [&](int i) { return slot_of(first + i); };
                     float *part = slot_of((int)blockIdx.x);
 #pragma unroll
                     for (int c = 0; c < D / 32; ++c) {
@@ -707,34 +719,37 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     if (shared) b_done();
                     part[32 * D + lane] = m;
                     part[32 * D + 32 + lane] = l;
-                    __threadfence();
-                    __syncwarp();
-                    int before = 0;
-                    if (lane == 0) {
-                        int *ticket = a.tickets + first * 8 + warp;
-                        before = atomicAdd(ticket, 1);
-                        if (before == parts - 1) *ticket = 0;  // zero again for the next launch
-                    }
-                    before = __shfl_sync(0xffffffffu, before, 0);
-                    __threadfence();
-                    write = before == parts - 1;
-                    if (write) {  // the last of the item's warps for these rows joins the parts, in the order of their keys
-                        float top = -INFINITY, sum = 0.0f;
+                    // whether this warp is the last of n to arrive at a counter; then the others' parts can be read
+                    auto last_of = [&](int *ticket, int n) {
+                        __threadfence();
+                        __syncwarp();
+                        int before = 0;
+                        if (lane == 0) {
+                            before = atomicAdd(ticket, 1);
+                            if (before == n - 1) *ticket = 0;  // zero again for the next launch
+                        }
+                        before = __shfl_sync(0xffffffffu, before, 0);
+                        __threadfence();
+                        return before == n - 1;
+                    };
+                    // joins parts of the CTAs from, from + step, ...: maximum and sum, then 32 columns at a time to `sink`
+                    auto join = [&](int from, int step, int n, float &top, float &sum, auto &&sink) {
+                        top = -INFINITY;
+                        sum = 0.0f;
 #pragma unroll 8
-                        for (int i = 0; i < parts; ++i) top = fmaxf(top, __ldcg(part_of(i) + 32 * D + lane));
+                        for (int i = 0; i < n; ++i) top = fmaxf(top, __ldcg(slot_of(from + i * step) + 32 * D + lane));
                         const float ref = top == -INFINITY ? 0.0f : top;
 #pragma unroll 4
-                        for (int i = 0; i < parts; ++i) {
-                            const float *pc = part_of(i) + 32 * D + lane;
+                        for (int i = 0; i < n; ++i) {
+                            const float *pc = slot_of(from + i * step) + 32 * D + lane;
                             sum = fmaf(__ldcg(pc + 32), fast_ex2((__ldcg(pc) - ref) * a.scale_log2), sum);
                         }
-                        inv = sum > 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll 1
                         for (int c = 0; c < D / 32; ++c) {
                             float v[32] = {};
 #pragma unroll 2
-                            for (int i = 0; i < parts; ++i) {
-                                const float *pc = part_of(i);
+                            for (int i = 0; i < n; ++i) {
+                                const float *pc = slot_of(from + i * step);
                                 const float g = fast_ex2((__ldcg(pc + 32 * D + lane) - ref) * a.scale_log2);
                                 float4 u[8];
 #pragma unroll
@@ -747,14 +762,46 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                                     v[4 * j + 3] = fmaf(u[j].w, g, v[4 * j + 3]);
                                 }
                             }
+                            sink(c, v);
+                        }
+                    };
+                    // Many parts are joined in two steps, groups first, since one warp reads a part in more than a microsecond.  A
+                    // CTA begins at most one shared item and continues at most one, so a counter per CTA, warp and use is enough.
+                    int span = 1, n = parts;
+                    bool go = true;
+                    if (parts > kJoinAtOnce) {
+                        span = (int)ceilf(sqrtf((float)parts));
+                        n = (parts + span - 1) / span;
+                        const int group = ((int)blockIdx.x - first) / span, from = first + group * span;
+                        const int members = min(span, final - from + 1);
+                        go = last_of(a.tickets + (from * 3 + (group == 0 ? 1 : 2)) * 8 + warp, members);
+                        if (go) {  // the group's parts become one, in the place of its first
+                            float top, sum;
+                            float *to_slot = slot_of(from);
+                            join(from, 1, members, top, sum, [&](int c, float(&v)[32]) {
+#pragma unroll
+                                for (int j = 0; j < 8; ++j)
+                                    *(reinterpret_cast<float4 *>(to_slot) + (8 * c + j) * 32 + lane) =
+                                        make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                            });
+                            to_slot[32 * D + lane] = top;
+                            to_slot[32 * D + 32 + lane] = sum;
+                        }
+                    }
+                    if (go && last_of(a.tickets + first * 3 * 8 + warp, n)) {
+                        // the last for these rows joins what there is, in the order of its keys
+                        write = true;
+                        float top, sum;
+                        join(first, span, n, top, sum, [&](int c, float(&v)[32]) {
+                            const float w = sum > 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
-                                *reinterpret_cast<uint4 *>(chunk_at(lane, 4 * c + i)) = make_uint4(
-                                    Half2Of<T>::pack(v[8 * i] * inv, v[8 * i + 1] * inv),
-                                    Half2Of<T>::pack(v[8 * i + 2] * inv, v[8 * i + 3] * inv),
-                                    Half2Of<T>::pack(v[8 * i + 4] * inv, v[8 * i + 5] * inv),
-                                    Half2Of<T>::pack(v[8 * i + 6] * inv, v[8 * i + 7] * inv));
-                        }
+                                *reinterpret_cast<uint4 *>(chunk_at(lane, 4 * c + i)) =
+                                    make_uint4(Half2Of<T>::pack(v[8 * i] * w, v[8 * i + 1] * w),
+                                               Half2Of<T>::pack(v[8 * i + 2] * w, v[8 * i + 3] * w),
+                                               Half2Of<T>::pack(v[8 * i + 4] * w, v[8 * i + 5] * w),
+                                               Half2Of<T>::pack(v[8 * i + 6] * w, v[8 * i + 7] * w));
+                        });
                     }
                 }
                 if (write) {
@@ -825,12 +872,7 @@ int make_page_map(CUtensorMap *map, void *base, const b200_w8a8_kv_cache *c, int
 template <typename T, int D>
 int launch_chunk(const CUtensorMap &k, const CUtensorMap &v, const AttnParams &a, const ChunkExtra &ex, int sms, bool &attr_set,
                  cudaStream_t stream) {
-    if (!attr_set) {
-        cudaError_t e = cudaFuncSetAttribute(attention_chunk_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             ChunkCfg<D>::kSmemBytes);
-        if (e != cudaSuccess) return fail("cudaFuncSetAttribute(attention_chunk): %s", cudaGetErrorString(e));
-        attr_set = true;
-    }
+    if (raise_smem_limit(attr_set, attention_chunk_kernel<T, D>, ChunkCfg<D>::kSmemBytes, "attention_chunk")) return 1;
     launch_kernel(attention_chunk_kernel<T, D>, dim3(sms), dim3(kChunkThreads), ChunkCfg<D>::kSmemBytes, stream, k, v, a, ex);
     return check_launch("paged_attention (chunk)");
 }
