@@ -215,7 +215,7 @@ def test_append(pkg, x, dtype, d, page, order, rope, by_position, norm, weights)
             assert torch.equal(k2[where], k_pages[where]) and torch.equal(v2[where], v_pages[where])
 
 
-@pytest.mark.parametrize("seqs,new", [(1, 2000), (300, 1), (1000, 3)])
+@pytest.mark.parametrize("seqs,new", [(1, 2000), (300, 1), (7, 101), (1000, 3), (5, 2603)])
 def test_append_many(pkg, seqs, new):
     """Every token at its place, many sequences or many tokens (values only: bit for bit)."""
     d, kv, page = 64, 3, 16
@@ -233,6 +233,34 @@ def test_append_many(pkg, seqs, new):
                   k, v)
     torch.cuda.synchronize()
     assert torch.equal(k_pages, want[0]) and torch.equal(v_pages, want[1])
+
+
+@pytest.mark.parametrize("x,d,rope", [("f32", 64, "SPLIT"), ("bf16", 128, "HALVES"), ("f16", 128, "PAIRS")])
+def test_append_in_parts(pkg, x, d, rope):
+    """However many rows a call has, and however its warps share them, a row comes out the same bit for bit."""
+    heads, kv, page, rows = 5, 3, 32, 13001
+    g = torch.Generator().manual_seed(d)
+    dtype = torch.float16 if x == "f16" else torch.bfloat16
+    k_pages, v_pages, table, _ = pr.make_cache([(rows, rows + 9)], page, kv, d, dtype, "tokens", g, DEV, fill=0.0)
+    src = torch.randn(rows, heads + 2 * kv, d, generator=g).to(pr.DTYPES[x]).to(DEV)
+    angle = torch.rand(rows + 9, d // 2, generator=g) * 6.3
+    kw = dict(norm_eps=1e-5, rope_order=getattr(pkg, "ROPE_" + rope), rope_cos=angle.cos().to(DEV), rope_sin=angle.sin().to(DEV),
+              rope_by_position=True)
+    got = {}
+    for part in (500, 2000, 11999, rows):
+        pools = [torch.zeros_like(k_pages), torch.zeros_like(v_pages)]
+        q_out = torch.zeros(rows, heads, d, dtype=dtype, device=DEV)
+        cache = pkg.PagedKVCache(*pools)
+        for a in range(0, rows, part):
+            b = min(rows, a + part)
+            batch = pkg.PagedBatch(table, torch.tensor([0, b - a], dtype=torch.int32, device=DEV),
+                                   torch.tensor([b + 9], dtype=torch.int32, device=DEV))
+            pkg.kv_append(cache, batch, src[a:b, heads:heads + kv], src[a:b, heads + kv:], q=src[a:b, :heads], q_out=q_out[a:b], **kw)
+        torch.cuda.synchronize()
+        assert pkg.poll_status() == 0
+        got[part] = (q_out, *pools)
+    for part in got:
+        assert all(torch.equal(a, b) for a, b in zip(got[part], got[rows])), part
 
 
 # ------------------------------------------------------------------ streams, graphs, errors

@@ -34,7 +34,7 @@ struct AppendParams {
     float eps;
     const float *q_weight, *k_weight, *cos, *sin;
     int by_position, rope_rows;
-    int warps_per_token;  // 1 or all of a CTA
+    int warps_per_token;  // 1, 2, 4 or all of a CTA
 };
 
 // The sequence whose new tokens hold row t, -1 if none does: the warp probes 32 starts at a time.
@@ -265,8 +265,15 @@ int kv_append(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *batch, 
     p.n_heads = x->q ? x->n_heads : 0;
     p.norm = x->norm != 0; p.eps = x->eps; p.q_weight = x->q_weight; p.k_weight = x->k_weight;
     p.cos = x->rope_cos; p.sin = x->rope_sin; p.by_position = x->rope_by_position != 0; p.rope_rows = x->rope_rows;
-    // fewer rows than 148 SMs x 4 CTAs x 8 warps hold (4736) leave warps without work: there the warps of a CTA share a row
-    p.warps_per_token = batch->n_tokens >= 4096 ? 1 : kAppendWarps;
+    // 148 SMs hold 4736 of these warps.  Few rows are spread over them, many are better off with a place looked up once and all
+    // heads of a row behind it.  Measured with 8 / 4 / 2 / 1 warps a row (64 heads of 64, fp16; 48 heads of 128, bf16), us:
+    //      512 rows   3.9 /  4.6 /  5.6 /  8.0
+    //     1024 rows   5.8 /  5.0 /  7.4 /  9.0      8.7 /  8.4 / 12.0 / 15.0
+    //     4096 rows  16.1 / 11.7 / 11.6 / 13.7     25.6 / 21.3 / 20.9 / 24.2
+    //     8192 rows  33.0 / 25.3 / 23.5 / 25.0     53.9 / 44.9 / 38.5 / 42.2
+    //    16384 rows  64.8 / 48.0 / 44.6 / 42.8    101.7 / 85.0 / 73.8 / 70.2
+    const int n = batch->n_tokens;
+    p.warps_per_token = n <= 592 ? kAppendWarps : n <= 2368 ? 4 : n <= 12000 ? 2 : 1;
     const int per_cta = kAppendWarps / p.warps_per_token;
     const unsigned grid = (unsigned)((batch->n_tokens + per_cta - 1) / per_cta);
     if (cache->dtype == B200_DT_F16) {
