@@ -247,7 +247,7 @@ def test_append_in_parts(pkg, x, d, rope):
     kw = dict(norm_eps=1e-5, rope_order=getattr(pkg, "ROPE_" + rope), rope_cos=angle.cos().to(DEV), rope_sin=angle.sin().to(DEV),
               rope_by_position=True)
     got = {}
-    for part in (500, 2000, 11999, rows):
+    for part in (500, 2000, 9001, rows):
         pools = [torch.zeros_like(k_pages), torch.zeros_like(v_pages)]
         q_out = torch.zeros(rows, heads, d, dtype=dtype, device=DEV)
         cache = pkg.PagedKVCache(*pools)

@@ -6,13 +6,13 @@
 //
 // Every element is read once and written once: memory bound.  A head's d elements are spread over d / 8 lanes, 16 bytes of
 // output each, so the sum of squares and the exchange of pairs that lie half a head apart are shuffles.  A warp takes whole
-// heads of one token, several at a time in flight, and reads the token's table entries once.  With many tokens a warp has a token
-// to itself; with few, the eight warps of a CTA share one.  Each warp finds its token's place by itself, while its first heads
-// are on the way: 32 probes at a time into the sequences' starts, then length and page; no barrier.
+// heads of one token, several at a time in flight, and reads the token's table entries once.  With many tokens a warp has a
+// token to itself; with few, two, four or the eight warps of a CTA share one.  Each warp finds its token's place by itself, while
+// its first heads are on the way: 32 probes at a time into the sequences' starts, then length and page; no barrier.
 //
-// Measured: 131072 fp16 rows (32 + 2 x 16 heads of 64) 295 us = 5.5 TB/s, 85 % of a plain copy (issue slots 62 % busy); a frame of
-// 512 fp32 rows 3.8 us, 128 bf16 rows of 128 sequences 4.9 us, one row 2.6 us.  With the tokens' places looked up by the CTA
-// behind barriers, and addresses and arithmetic element by element, the first took 327 us; without the heads in flight 401 us.
+// Measured: 98348 fp16 rows (32 + 2 x 16 heads of 64) 287 to 295 us = 5.6 TB/s, 86 % of a plain copy (issue slots 62 % busy); a
+// frame of 512 fp32 rows 3.8 us, 128 bf16 rows of 128 sequences 4.9 us, one row 2.6 us.  With the places looked up by the CTA
+// behind barriers, and addresses and arithmetic element by element, the first took 327 us; without several heads in flight 401.
 #include "paged_kv.cuh"
 
 namespace b200 {
@@ -194,7 +194,8 @@ __global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(const Appe
 #pragma unroll
             for (int j = 0; j < 4; ++j) unpair2(x[j], a[j], b[j]);
             if (ROPE == B200_ROPE_SPLIT && !is_v) {
-                *reinterpret_cast<uint2 *>(dst + lane * 4) = make_uint2(Half2Of<TC>::pack(a[0], a[1]), Half2Of<TC>::pack(a[2], a[3]));
+                *reinterpret_cast<uint2 *>(dst + lane * 4) =
+                    make_uint2(Half2Of<TC>::pack(a[0], a[1]), Half2Of<TC>::pack(a[2], a[3]));
                 *reinterpret_cast<uint2 *>(dst + D / 2 + lane * 4) =
                     make_uint2(Half2Of<TC>::pack(b[0], b[1]), Half2Of<TC>::pack(b[2], b[3]));
             } else {
@@ -209,10 +210,10 @@ __global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(const Appe
 template <typename TX, typename TC, int D>
 cudaError_t launch_append(const AppendParams &p, int rope, dim3 grid, cudaStream_t st) {
     switch (rope) {
-        case B200_ROPE_SPLIT: return launch_kernel(kv_append_kernel<TX, TC, D, B200_ROPE_SPLIT>, grid, dim3(kAppendThreads), 0, st, p);
-        case B200_ROPE_HALVES: return launch_kernel(kv_append_kernel<TX, TC, D, B200_ROPE_HALVES>, grid, dim3(kAppendThreads), 0, st, p);
-        case B200_ROPE_PAIRS: return launch_kernel(kv_append_kernel<TX, TC, D, B200_ROPE_PAIRS>, grid, dim3(kAppendThreads), 0, st, p);
-        default: return launch_kernel(kv_append_kernel<TX, TC, D, B200_ROPE_NONE>, grid, dim3(kAppendThreads), 0, st, p);
+        case B200_ROPE_SPLIT: return launch_kernel(kv_append_kernel<TX, TC, D, B200_ROPE_SPLIT>, grid, kAppendThreads, 0, st, p);
+        case B200_ROPE_HALVES: return launch_kernel(kv_append_kernel<TX, TC, D, B200_ROPE_HALVES>, grid, kAppendThreads, 0, st, p);
+        case B200_ROPE_PAIRS: return launch_kernel(kv_append_kernel<TX, TC, D, B200_ROPE_PAIRS>, grid, kAppendThreads, 0, st, p);
+        default: return launch_kernel(kv_append_kernel<TX, TC, D, B200_ROPE_NONE>, grid, kAppendThreads, 0, st, p);
     }
 }
 template <typename TC, int D>
@@ -267,13 +268,14 @@ int kv_append(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *batch, 
     p.cos = x->rope_cos; p.sin = x->rope_sin; p.by_position = x->rope_by_position != 0; p.rope_rows = x->rope_rows;
     // 148 SMs hold 4736 of these warps.  Few rows are spread over them, many are better off with a place looked up once and all
     // heads of a row behind it.  Measured with 8 / 4 / 2 / 1 warps a row (64 heads of 64, fp16; 48 heads of 128, bf16), us:
-    //      512 rows   3.9 /  4.6 /  5.6 /  8.0
-    //     1024 rows   5.8 /  5.0 /  7.4 /  9.0      8.7 /  8.4 / 12.0 / 15.0
-    //     4096 rows  16.1 / 11.7 / 11.6 / 13.7     25.6 / 21.3 / 20.9 / 24.2
-    //     8192 rows  33.0 / 25.3 / 23.5 / 25.0     53.9 / 44.9 / 38.5 / 42.2
-    //    16384 rows  64.8 / 48.0 / 44.6 / 42.8    101.7 / 85.0 / 73.8 / 70.2
+    //      400 rows   3.9 /  4.6 /  5.6 /  8.0
+    //      800 rows   5.8 /  5.0 /  7.4 /  9.0      8.7 /  8.4 / 12.0 / 15.0
+    //     1600 rows   8.8 /  7.4 /  7.9 / 12.6     13.6 / 13.0 / 13.3 / 21.1
+    //     3200 rows  16.1 / 11.7 / 11.6 / 13.7     25.6 / 21.3 / 20.9 / 24.2
+    //     6400 rows  33.0 / 25.3 / 23.5 / 25.0     53.9 / 44.9 / 38.5 / 42.2
+    //    12500 rows  64.8 / 48.0 / 44.6 / 42.8    101.7 / 85.0 / 73.8 / 70.2
     const int n = batch->n_tokens;
-    p.warps_per_token = n <= 592 ? kAppendWarps : n <= 2368 ? 4 : n <= 12000 ? 2 : 1;
+    p.warps_per_token = n <= 592 ? kAppendWarps : n <= 2368 ? 4 : n <= 9472 ? 2 : 1;
     const int per_cta = kAppendWarps / p.warps_per_token;
     const unsigned grid = (unsigned)((batch->n_tokens + per_cta - 1) / per_cta);
     if (cache->dtype == B200_DT_F16) {

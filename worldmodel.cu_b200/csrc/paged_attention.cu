@@ -11,7 +11,7 @@
 //
 // Measured: 64 sequences of up to 8191 keys (32 / 8 heads of 128, bf16) 246 us = 6.5 TB/s, what a plain copy reaches; one of
 // 131071 keys 94 us = 5.7 TB/s (of the rest about 5 us are launch, plan and first loads, 4 us the join); one of 777 keys
-// (32 / 16 heads of 64) 9.6 us, all latency: plan 1.8, queries and first keys 1.3, keys 1.5, parts and counter 1.4, join 2.3.
+// (32 / 16 heads of 64) 9.6 us, all latency: plan, first loads, parts and join, each behind the one before.
 #include <algorithm>
 #include <mutex>
 
@@ -24,7 +24,9 @@ constexpr int kRowsThreads = 128;
 constexpr int kRowTile = 16;  // rows of one matrix instruction
 constexpr int kStepKeys = 16;
 constexpr int kRowsKeyTile = kStepKeys * (kRowsThreads / 32);  // keys per KV tile of the plan
-constexpr int kRowsExtra = 2;  // measured 0 / 2 / 5: one of 777 keys 12.7 / 11.2 / 10.3 us, one of 131071 keys 95.8 / 94.0 / 93.3 us
+// measured 0 / 2 / 5: one sequence of 777 keys 12.7 / 11.2 / 10.3 us (more units, so more parts, which min_tiles below gives it
+// as well), one of 131071 keys 95.8 / 94.0 / 93.3 us
+constexpr int kRowsExtra = 2;
 
 template <int D>
 struct RowsCfg {

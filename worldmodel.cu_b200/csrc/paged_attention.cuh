@@ -39,7 +39,7 @@ struct AttnParams {
     FastDiv by_group, by_block, by_heads;  // by_block: of 1 where block is 0; by_heads: of the key heads
     float scale_log2;  // scale * log2(e): weights are 2^(scale_log2 * (s - max))
     int block, window;
-    int min_tiles;     // no CTA gets fewer KV tiles than this while others have none
+    int min_tiles;     // no CTA gets fewer units than this while others have none
     int *tickets;
     float *partials;
 };

@@ -71,8 +71,9 @@ __device__ __forceinline__ bool elect_one() {
         : "=r"(one));
     return one != 0;
 }
-// Four products over 16 elements of K each: 32 bytes of a K-major row, or 8 columns of weights and 16 rows of values.  One block of assembly with its own arithmetic: left to the compiler, the operands of all unrolled products are
-// kept in registers that the issuing warp does not have.
+// Four products over 16 elements of K each: 32 bytes of a K-major row, or 8 columns of weights and 16 rows of values.  One block
+// of assembly with its own arithmetic: left to the compiler, the operands of all unrolled products are kept in registers that the
+// issuing warp does not have.
 __device__ __forceinline__ void umma_f16_ss4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
         "{\n\t.reg .pred p, t;\n\t.reg .b64 a, b;\n\t"
@@ -314,7 +315,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     const unsigned mask = __ballot_sync(0xffffffffu, live);
                     const uint32_t bytes = (uint32_t)__popc(mask) * (uint32_t)ex.page_box * (D * 2);
                     for (int kv = 0; kv < 2; ++kv) {
-                        ok = __all_sync(0xffffffffu, wait_bounded(kv_empty + 8 * s, ph ^ 1u, abort_flag, ex.wait_tries, KS_TIMEOUT_SMEM_EMPTY));
+                        ok = wait_bounded(kv_empty + 8 * s, ph ^ 1u, abort_flag, ex.wait_tries, KS_TIMEOUT_SMEM_EMPTY);
+                        ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                         if (lane == 0) mbar_arrive_expect_tx(bars + s, bytes);
                         __syncwarp();
@@ -506,7 +508,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     visible_keys(a, it.seq.keys - it.seq.n + a.by_group.div(row0 + lane), it.seq.keys, lo, hi);
                 const int lo_max = __reduce_max_sync(0xffffffffu, lo), hi_min = __reduce_min_sync(0xffffffffu, hi);
                 for (int kt = kt_first; kt < kt1; kt += kt_step) {
-                    ok = __all_sync(0xffffffffu, wait_bounded(s_full + 8 * tile, s_ph, abort_flag, ex.wait_tries, KS_TIMEOUT_SOFTMAX));
+                    ok = wait_bounded(s_full + 8 * tile, s_ph, abort_flag, ex.wait_tries, KS_TIMEOUT_SOFTMAX);
+                    ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     s_ph ^= 1u;
                     tc_fence_after_sync();
@@ -634,14 +637,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     stats[32 + lane] = l;
                     __syncwarp();
                     if (lane == 0) arrive_on(b_known + 8 * sub);
-                    ok = __all_sync(0xffffffffu, wait_bounded(b_taken + 8 * sub, known_ph, abort_flag, ex.wait_tries, KS_TIMEOUT_TMEM_FULL));
+                    ok = wait_bounded(b_taken + 8 * sub, known_ph, abort_flag, ex.wait_tries, KS_TIMEOUT_TMEM_FULL);
+                    ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     known_ph ^= 1u;
                     if (mine_any) o_ph ^= 1u;
                     if (more) load_q(it.rt * kChunkRows + tile * 128 + sub * 32);
                     continue;
                 }
-                ok = __all_sync(0xffffffffu, wait_bounded(o_full + 8 * tile, o_ph, abort_flag, ex.wait_tries, KS_TIMEOUT_TMEM_FULL));
+                ok = wait_bounded(o_full + 8 * tile, o_ph, abort_flag, ex.wait_tries, KS_TIMEOUT_TMEM_FULL);
+                ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 o_ph ^= 1u;
                 // this row's factors of the two accumulators
