@@ -399,9 +399,9 @@ int b200_w8a8_kv_append(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batc
  * Scores, softmax and sums are fp32; weights are rounded to the cache's type for the product with the values.
  * scale must be positive and finite, n_heads a multiple of the cache's n_kv_heads.
  * workspace: at least b200_w8a8_paged_attention_workspace_size bytes on the current device, 256-byte aligned, its first
- * 32768 bytes zero before the first call; every call leaves them zero.  Calls that may overlap on the GPU (graphs replayed
- * on different streams too) need a workspace each.  Stands in for the reference's attention over its ring
- * (src/world_cuda.cu:1960-2056). */
+ * 32768 bytes zero before the first call; every call leaves them zero, except one whose wait ran out: zero them again
+ * then.  Calls that may overlap on the GPU (graphs replayed on different streams too) need a workspace each.  Stands in
+ * for the reference's attention over its ring (src/world_cuda.cu:1960-2056). */
 size_t b200_w8a8_paged_attention_workspace_size(int d_head);
 int b200_w8a8_paged_attention(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *batch, const void *q,
                               int64_t q_token_stride, int64_t q_head_stride, void *out, int64_t out_token_stride,
