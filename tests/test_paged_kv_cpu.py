@@ -119,3 +119,10 @@ def test_the_bounds_of_the_reference_hold_for_a_plain_rounded_evaluation():
         e = (s.masked_fill(~mask, -float("inf")) - s.masked_fill(~mask, -float("inf")).amax(-1, keepdim=True)).exp()
         o = torch.einsum("hnk,khd->nhd", e.to(dtype).float(), vv) / e.sum(-1).T[..., None]
         assert bool(((o.to(dtype).double() - want).abs() <= bound).all())
+
+
+def test_arguments_packed_as_bytes_have_the_structures_layout(pkg):
+    batch = (11, 12, 13, 4, 5, 6, 7)
+    assert pkg._pack_batch(*batch) == bytes(pkg._Batch(*batch))
+    new = (21, 22, 23, 1, 2, 3, 4, 5, 6, 1, 32, 24, 7, 8, 1, 1e-5, 25, 26, 2, 27, 28, 1, 99)
+    assert pkg._pack_new(*new) == bytes(pkg._New(*new))

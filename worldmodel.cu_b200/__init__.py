@@ -13,6 +13,7 @@ The directory name contains a dot, so it is not importable by name; load it with
 from __future__ import annotations
 
 import ctypes
+import struct
 from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p, POINTER
 from pathlib import Path
 
@@ -148,9 +149,14 @@ def _stream():
     return torch.cuda.current_stream().cuda_stream
 
 
+_dt_codes = {}
+
+
 def _dt(t) -> int:
-    import torch
-    return {torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16, torch.int32: DT_S32}[t.dtype]
+    if not _dt_codes:
+        import torch
+        _dt_codes.update({torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16, torch.int32: DT_S32})
+    return _dt_codes[t.dtype]
 
 
 def mma_rate(slabs_per_cta=16384) -> float:
@@ -471,6 +477,10 @@ class _New(ctypes.Structure):
                 ("rope_sin", c_void_p), ("rope_by_position", c_int), ("rope_rows", c_int)]
 
 
+# the last two as bytes of the same layout, made in a fifth of the time that filling a ctypes structure takes
+_pack_batch, _pack_new = struct.Struct("@3P4i").pack, struct.Struct("@3P6q2iP2qif2Pi2P2i").pack
+
+
 def _require(ok, what):
     if not ok:
         raise W8A8Error(what)
@@ -512,8 +522,8 @@ class PagedBatch:
         self.fields = (page_table.data_ptr(), q_starts.data_ptr(), kv_lens.data_ptr(), seqs, page_table.shape[1])
 
     def of(self, n_tokens):
-        """The struct for row buffers of n_tokens rows, one for every call."""
-        return ctypes.byref(_Batch(*self.fields, n_tokens, n_tokens if self.max_new_tokens is None else self.max_new_tokens))
+        """The struct for row buffers of n_tokens rows, as bytes, one for every call."""
+        return _pack_batch(*self.fields, n_tokens, n_tokens if self.max_new_tokens is None else self.max_new_tokens)
 
 
 _raw_stream = None  # torch's stream look-up without building a Stream object, where this torch has it
@@ -533,15 +543,16 @@ def _call_on(index, fn):
 
 
 def _heads_strides(t, what, index, d_head):
-    """Token and head stride of a [tokens, heads, d_head] tensor on device `index`."""
-    if t.dim() != 3 or t.shape[2] != d_head:
-        raise W8A8Error(f"{what} is [tokens, heads, d_head]: got {tuple(t.shape)} for d_head {d_head}")
+    """Shape, token and head stride of a [tokens, heads, d_head] tensor on device `index`."""
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != d_head:
+        raise W8A8Error(f"{what} is [tokens, heads, d_head]: got {tuple(shape)} for d_head {d_head}")
     ts, hs, one = t.stride()
     if one != 1:
         raise W8A8Error(f"{what}'s last dimension is contiguous")
     if t.get_device() != index:
         raise W8A8Error(f"all tensors of a call are on the cache's device: {what} is not")
-    return ts, hs
+    return shape, ts, hs
 
 
 def kv_append(cache, batch, k, v, q=None, q_out=None, norm_eps=None, q_weight=None, k_weight=None, rope_cos=None,
@@ -551,22 +562,23 @@ def kv_append(cache, batch, k, v, q=None, q_out=None, norm_eps=None, q_weight=No
     queries and keys on the way.  k, v, q: [tokens, heads, d_head] of one type (fp32, fp16, bf16), any strides that are
     multiples of 16 bytes."""
     import torch
-    d, index, n, dtype = cache.d_head, cache.index, k.shape[0], k.dtype
-    kt, kh = _heads_strides(k, "k", index, d)
-    vt, vh = _heads_strides(v, "v", index, d)
-    if k.shape != v.shape or v.dtype != dtype or k.shape[1] != cache.n_kv_heads:
-        raise W8A8Error(f"k and v are [tokens, {cache.n_kv_heads}, {d}] of one type: got {tuple(k.shape)} and {tuple(v.shape)}")
+    d, index, dtype = cache.d_head, cache.index, k.dtype
+    shape, kt, kh = _heads_strides(k, "k", index, d)
+    v_shape, vt, vh = _heads_strides(v, "v", index, d)
+    n = shape[0]
+    if shape != v_shape or v.dtype != dtype or shape[1] != cache.n_kv_heads:
+        raise W8A8Error(f"k and v are [tokens, {cache.n_kv_heads}, {d}] of one type: got {tuple(shape)} and {tuple(v_shape)}")
     if batch.index != index:
         raise W8A8Error("all tensors of a call are on the cache's device: the batch's are not")
     qp = qt = qh = op = ot = oh = heads = 0
     if q is not None:
-        qt, qh = _heads_strides(q, "q", index, d)
+        q_shape, qt, qh = _heads_strides(q, "q", index, d)
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=cache.dtype, device=q.device)
-        ot, oh = _heads_strides(q_out, "q_out", index, d)
-        if q.shape[0] != n or q.dtype != dtype or q_out.shape != q.shape or q_out.dtype != cache.dtype:
+            q_out = torch.empty(q_shape, dtype=cache.dtype, device=q.device)
+        out_shape, ot, oh = _heads_strides(q_out, "q_out", index, d)
+        if q_shape[0] != n or q.dtype != dtype or out_shape != q_shape or q_out.dtype != cache.dtype:
             raise W8A8Error("q has k's rows and type, q_out q's shape and the cache's type")
-        qp, op, heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
+        qp, op, heads = q.data_ptr(), q_out.data_ptr(), q_shape[1]
     elif q_out is not None:
         raise W8A8Error("q_out without q")
     for w in (q_weight, k_weight):
@@ -577,13 +589,15 @@ def kv_append(cache, batch, k, v, q=None, q_out=None, norm_eps=None, q_weight=No
         if rope_cos is None or rope_sin is None:
             raise W8A8Error("a rotation needs rope_cos and rope_sin")
         rows = rope_cos.shape[0]
+        want = (rows, d // 2)
         for t in (rope_cos, rope_sin):
-            if t.dtype != torch.float32 or t.shape != (rows, d // 2) or not t.is_contiguous() or t.get_device() != index:
+            if t.dtype != torch.float32 or t.shape != want or not t.is_contiguous() or t.get_device() != index:
                 raise W8A8Error("rope_cos and rope_sin are contiguous fp32 [rows, d_head / 2] on the cache's device")
         cp, sp = rope_cos.data_ptr(), rope_sin.data_ptr()
-    x = _New(qp, k.data_ptr(), v.data_ptr(), qt, qh, kt, kh, vt, vh, _dt(k), heads, op, ot, oh, norm_eps is not None,
-             norm_eps or 0.0, _ptr(q_weight), _ptr(k_weight), rope_order or 0, cp, sp, rope_by_position, rows)
-    _check(_call_on(index, lambda st: lib().b200_w8a8_kv_append(cache.ref, batch.of(n), ctypes.byref(x), st)), "kv_append")
+    x = _pack_new(qp, k.data_ptr(), v.data_ptr(), qt, qh, kt, kh, vt, vh, _dt(k), heads, op, ot, oh, norm_eps is not None,
+                  norm_eps or 0.0, 0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(),
+                  rope_order or 0, cp, sp, bool(rope_by_position), rows)
+    _check(_call_on(index, lambda st: lib().b200_w8a8_kv_append(cache.ref, batch.of(n), x, st)), "kv_append")
     return q_out
 
 
@@ -602,17 +616,17 @@ def paged_attention(q, cache, batch, scale=None, causal_block=1, window=0, out=N
     scale: 1 / sqrt(d_head) when None.  workspace: from make_attention_workspace (a fresh one when None)."""
     import torch
     d, index = cache.d_head, cache.index
-    qt, qh = _heads_strides(q, "q", index, d)
+    shape, qt, qh = _heads_strides(q, "q", index, d)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ot, oh = _heads_strides(out, "out", index, d)
-    if q.dtype != cache.dtype or out.dtype != q.dtype or out.shape != q.shape:
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    out_shape, ot, oh = _heads_strides(out, "out", index, d)
+    if q.dtype != cache.dtype or out.dtype != cache.dtype or out_shape != shape:
         raise W8A8Error("q has the cache's type, out q's shape and type")
     if workspace is None:
         workspace = make_attention_workspace(cache)
     if batch.index != index or workspace.get_device() != index:
         raise W8A8Error("all tensors of a call are on the cache's device: the batch's or the workspace is not")
-    n, heads, _ = q.shape
+    n, heads, _ = shape
     _check(_call_on(index, lambda st: lib().b200_w8a8_paged_attention(
         cache.ref, batch.of(n), q.data_ptr(), qt, qh, out.data_ptr(), ot, oh, heads, d ** -0.5 if scale is None else scale,
         causal_block, window, workspace.data_ptr(), workspace.nbytes, st)), "paged_attention")
