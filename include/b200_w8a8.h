@@ -378,7 +378,7 @@ typedef struct {
     int rope_order;               /* B200_ROPE_* */
     const float *rope_cos, *rope_sin; /* [rope_rows, d_head / 2], dense */
     int rope_by_position;         /* 0: row of the tables = row of the token; 1: row = position of the token */
-    int rope_rows;
+    int rope_rows;                /* a token beyond them is not appended, and reported like a page outside the cache */
 } b200_w8a8_kv_new;
 
 /* Norm and rotation of the new queries and keys in fp32, one rounding to the cache's type; keys and values go to their

@@ -129,3 +129,19 @@ def test_refusals(pkg):
     with pytest.raises(pkg.W8A8Error, match="workspace"):
         drv.forward_paged(packed, tokens, cos, cos, cache, batch, workspace=torch.zeros(256, dtype=torch.uint8, device=DEV))
     drv.close()
+
+
+def test_a_refused_layer_leaves_the_cache_alone(pkg):
+    """What the attention would refuse is refused before keys and values are written."""
+    T, D, HQ, HKV, DH, HID = 32, 256, 4, 2, 64, 512
+    L, layout, cache, table, drv, g = setup(pkg, T, D, HQ, HKV, DH, HID, True, False, 16, torch.float16, 1)
+    batch = pkg.PagedBatch(table, torch.tensor([0, T], dtype=torch.int32, device=DEV), torch.tensor([T], dtype=torch.int32, device=DEV))
+    tokens, cos, packed = torch.ones(T, D, device=DEV), torch.ones(T, DH // 2, device=DEV), drv.pack(L)
+    small = torch.zeros(256, dtype=torch.uint8, device=DEV)
+    for kw, match in ((dict(causal_block=0, window=5), "window"), (dict(causal_block=-1), "causal_block"), (dict(workspace=small), "workspace")):
+        with pytest.raises(pkg.W8A8Error, match=match):
+            drv.forward_paged(packed, tokens, cos, cos, cache, batch, **kw)
+    torch.cuda.synchronize()
+    assert bool(cache.k_pages.isnan().all()) and bool(cache.v_pages.isnan().all())
+    assert bool(drv.forward_paged(packed, tokens, cos, cos, cache, batch).isfinite().all())
+    drv.close()

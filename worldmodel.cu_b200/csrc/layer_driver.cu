@@ -189,6 +189,9 @@ int b200_w8a8_layer_forward_paged(void *handle, const b200_w8a8_layer *L, const 
     if (cache->n_kv_heads != c->n_kv_heads || cache->d_head != dh)
         return fail("layer_forward_paged: the cache has %d heads of %d, the layer %d of %d", cache->n_kv_heads, cache->d_head,
                     c->n_kv_heads, dh);
+    // what the attention refuses is refused before the cache is written
+    const float scale = 1.0f / sqrtf((float)dh);
+    if (check_paged_attention(cache, batch, c->n_heads, scale, causal_block, window, workspace, workspace_bytes)) return 1;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     // the two 16-bit [T, d] buffers fill the fp32 one that the controller's result needs only later
     char *q16 = reinterpret_cast<char *>(c->xc), *attn = q16 + (size_t)T * d * 2;
@@ -205,8 +208,8 @@ int b200_w8a8_layer_forward_paged(void *handle, const b200_w8a8_layer *L, const 
         return 1;
     if (run_linear(c, L->w_qkv, L->s_qkv, c->n_qkv, d, nullptr, nullptr, nullptr, B200_ACT_NONE, c->h, T, st)) return 1;
     if (kv_append(cache, batch, &x, st)) return 1;
-    if (paged_attention(cache, batch, q16, d, dh, attn, d, dh, c->n_heads, 1.0f / sqrtf((float)dh), causal_block, window,
-                        workspace, workspace_bytes, st))
+    if (paged_attention(cache, batch, q16, d, dh, attn, d, dh, c->n_heads, scale, causal_block, window, workspace,
+                        workspace_bytes, st))
         return 1;
     return after_attention(c, L, attn, cache->dtype, tokens, tokens_next, T, st);
 }

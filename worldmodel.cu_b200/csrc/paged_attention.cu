@@ -395,9 +395,17 @@ size_t paged_attention_workspace_size(int d_head) {
     return workspace_bytes_for(d_head, std::min(current_device_sms(dev), kMaxSms));
 }
 
-int paged_attention(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *batch, const void *q, long long q_ts,
-                    long long q_hs, void *out, long long o_ts, long long o_hs, int n_heads, float scale, int causal_block,
-                    int window, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
+// At most so many units of work; the kernels count them in 32 bits.
+static bool work_fits(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *batch, int group, int row_tile, int key_tile,
+                      int extra) {
+    const double rows = (double)batch->n_tokens * group / row_tile + batch->n_seqs;
+    const double keys = (double)batch->max_pages * cache->page_tokens / key_tile + 1 + extra;
+    return rows * keys * cache->n_kv_heads < 2147483000.0;
+}
+
+// What a call refuses whatever its rows; 1 after a message.
+int check_paged_attention(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *batch, int n_heads, float scale,
+                          int causal_block, int window, const void *workspace, size_t workspace_bytes) {
     if (const char *why = check_paged_cache(cache, batch)) return fail("paged_attention: %s", why);
     if (n_heads <= 0 || n_heads % cache->n_kv_heads != 0)
         return fail("paged_attention: %d heads are no multiple of the cache's %d", n_heads, cache->n_kv_heads);
@@ -405,15 +413,27 @@ int paged_attention(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *b
     if (causal_block < 0 || window < 0 || (window > 0 && causal_block == 0))
         return fail("paged_attention: causal_block=%d window=%d (a window needs causal_block)", causal_block, window);
     if (batch->n_tokens == 0 || batch->n_seqs == 0) return 0;
+    if (((long long)batch->n_tokens * n_heads) >> 30) return fail("paged_attention: n_tokens * n_heads must stay below 2^30");
+    const size_t need = paged_attention_workspace_size(cache->d_head);
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < need)
+        return fail("paged_attention needs a 256-byte aligned workspace of %zu bytes, got %zu", need,
+                    workspace ? workspace_bytes : (size_t)0);
+    if (!work_fits(cache, batch, n_heads / cache->n_kv_heads, kChunkRows, kKeyTile, kChunkExtra))
+        return fail("paged_attention: %d new tokens over up to %lld keys are too much for one call; pass fewer at a time",
+                    batch->n_tokens, (long long)batch->max_pages * cache->page_tokens);
+    return 0;
+}
+
+int paged_attention(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *batch, const void *q, long long q_ts,
+                    long long q_hs, void *out, long long o_ts, long long o_hs, int n_heads, float scale, int causal_block,
+                    int window, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
+    if (check_paged_attention(cache, batch, n_heads, scale, causal_block, window, workspace, workspace_bytes)) return 1;
+    if (batch->n_tokens == 0 || batch->n_seqs == 0) return 0;
     if (!q || !out) return fail("paged_attention: null q or out");
     if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) || ((q_ts | q_hs | o_ts | o_hs) & 7))
         return fail("paged_attention needs 16-byte aligned q and out and strides that are multiples of 8 elements");
-    if (((long long)batch->n_tokens * n_heads) >> 30) return fail("paged_attention: n_tokens * n_heads must stay below 2^30");
     int dev;
     const int sms = std::min(current_device_sms(dev), kMaxSms);
-    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < workspace_bytes_for(cache->d_head, sms))
-        return fail("paged_attention needs a 256-byte aligned workspace of %zu bytes, got %zu",
-                    workspace_bytes_for(cache->d_head, sms), workspace ? workspace_bytes : (size_t)0);
     AttnParams a{};
     a.c = make_view(cache, batch);
     a.q = q; a.q_ts = q_ts; a.q_hs = q_hs;
@@ -429,22 +449,12 @@ int paged_attention(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *b
     a.partials = reinterpret_cast<float *>(reinterpret_cast<char *>(workspace) + kTicketBytes);
     AttnDeviceInfo &di = attn_device_info(dev);
     const bool bf = cache->dtype == B200_DT_BF16;
-    // at most so many units of work; the kernels count them in 32 bits
-    auto work_fits = [&](long long row_tile, long long key_tile, long long extra) {
-        const double rows = (double)batch->n_tokens * a.group / row_tile + batch->n_seqs;
-        const double keys = (double)batch->max_pages * cache->page_tokens / key_tile + 1 + extra;
-        return rows * keys * cache->n_kv_heads < 2147483000.0;
-    };
     // One row tile of 16 rows: the rows kernel, bound by HBM whatever the group.  More rows would read every key again for each
     // row tile: measured with 20, 32 and 48 rows, the chunk kernel / the rows kernel, 53.5 / 52.0, 36.3 / 42.5 and 85 / 160 us.
-    if ((long long)batch->max_new_tokens * a.group > kRowTile || !work_fits(kRowTile, kRowsKeyTile, kRowsExtra)) {
-        if (!work_fits(256, 128, 3))
-            return fail("paged_attention: %d new tokens over up to %lld keys are too much for one call; pass fewer at a time",
-                        batch->n_tokens, (long long)batch->max_pages * cache->page_tokens);
-        a.min_tiles = 2;
-        return launch_attention_chunk(cache, a, sms, dev, stream);
-    }
+    const bool few = (long long)batch->max_new_tokens * a.group <= kRowTile;
     a.min_tiles = 2;  // measured 2 / 4 / 8 / 16 units at least: one sequence of 777 keys 9.7 / 11.2 / 13.8 / 18.9 us
+    if (!few || !work_fits(cache, batch, a.group, kRowTile, kRowsKeyTile, kRowsExtra))
+        return launch_attention_chunk(cache, a, sms, dev, stream);
     if (cache->d_head == 64)
         return bf ? launch_rows<__nv_bfloat16, 64>(a, sms, di.attr_set[0][1], stream)
                   : launch_rows<__half, 64>(a, sms, di.attr_set[0][0], stream);

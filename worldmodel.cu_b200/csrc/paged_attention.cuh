@@ -50,6 +50,12 @@ int launch_attention_chunk(const b200_w8a8_kv_cache *cache, const AttnParams &a,
 
 namespace {
 
+// of the chunk kernel, whose units of work the entry counts too
+constexpr int kChunkRows = 256;  // two row tiles
+constexpr int kKeyTile = 128;
+// EXTRA, measured 1 / 2 / 3 / 5 / 8: the prompt 659 / 532 / 469 / 474 / 487 us (its first CTA has 50 items of one to four tiles), 80 rows
+// of 16 sequences 33.5 / 31.6 / 30.6 / 29.3 / 28.9 us, the frame 64.5 / 64.0 / 62.9 / 64.1 / 65.5 us
+constexpr int kChunkExtra = 3;
 constexpr int kTicketBytes = 32768;                // counters at the start of the workspace
 constexpr int kMaxSms = kTicketBytes / 4 / (8 * 3);  // the chunk kernel's joining warps have three each
 

@@ -31,11 +31,6 @@ namespace {
 constexpr int kChunkThreads = 384;  // three warpgroups; warps 10 and 11 only fill the third
 // registers a thread: 384 x 168 at launch = 64512 = 256 x 224 + 128 x 56
 constexpr int kSoftmaxRegs = 224, kOtherRegs = 56;
-constexpr int kChunkRows = 256;   // two row tiles
-constexpr int kKeyTile = 128;
-// measured 1 / 2 / 3 / 5 / 8: the prompt 659 / 532 / 469 / 474 / 487 us (its first CTA has 50 items of one to four tiles), 80 rows
-// of 16 sequences 33.5 / 31.6 / 30.6 / 29.3 / 28.9 us, the frame 64.5 / 64.0 / 62.9 / 64.1 / 65.5 us
-constexpr int kChunkExtra = 3;
 constexpr int kSlabBytes = 128 * 128;  // 128 rows of 64 16-bit elements, 128-byte swizzle
 constexpr float kLazyRescale = 8.0f;   // log2 of how far a weight may exceed one
 constexpr int kJoinAtOnce = 8;         // parts of an item that are joined in one step

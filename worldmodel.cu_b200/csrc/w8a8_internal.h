@@ -206,6 +206,8 @@ int gemm_forced_tile_width();  // 0 unless a test forced one
 int kv_append(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *batch, const b200_w8a8_kv_new *tokens,
               cudaStream_t stream);
 size_t paged_attention_workspace_size(int d_head);
+int check_paged_attention(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *batch, int n_heads, float scale,
+                          int causal_block, int window, const void *workspace, size_t workspace_bytes);
 int paged_attention(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *batch, const void *q, long long q_ts,
                     long long q_hs, void *out, long long o_ts, long long o_hs, int n_heads, float scale, int causal_block,
                     int window, void *workspace, size_t workspace_bytes, cudaStream_t stream);
