@@ -450,7 +450,7 @@ int paged_attention(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *b
     AttnDeviceInfo &di = attn_device_info(dev);
     const bool bf = cache->dtype == B200_DT_BF16;
     // One row tile of 16 rows: the rows kernel, bound by HBM whatever the group.  More rows would read every key again for each
-    // row tile: measured with 20, 32 and 48 rows, the chunk kernel / the rows kernel, 53.5 / 52.0, 36.3 / 42.5 and 85 / 160 us.
+    // row tile: measured with 20, 32 and 48 rows, the chunk kernel / the rows kernel, 49.7 / 52.0, 35.1 / 42.5 and 84 / 160 us.
     const bool few = (long long)batch->max_new_tokens * a.group <= kRowTile;
     a.min_tiles = 2;  // measured 2 / 4 / 8 / 16 units at least: one sequence of 777 keys 9.7 / 11.2 / 13.8 / 18.9 us
     if (!few || !work_fits(cache, batch, a.group, kRowTile, kRowsKeyTile, kRowsExtra))

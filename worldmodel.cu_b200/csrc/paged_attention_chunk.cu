@@ -12,7 +12,8 @@
 // An item of at most 128 rows has no second row tile: both accumulators work on it, KV tiles in turn.
 //
 // Measured: a prompt of 8192 tokens (32 / 8 heads of 128, bf16, causal) 470 us = 1.17 PFLOP/s, 71 % of the rate of a large
-// library product; a frame of 512 tokens over 8704 keys (32 / 16 heads of 64, fp16) 63 us.  The tensor pipe is busy 56 % of the
+// library product; a frame of 512 tokens over 8704 keys (32 / 16 heads of 64, fp16) 62.5 us,
+// 80 rows of 16 sequences of up to 4001 keys (32 / 2 heads of 128) 27.9 us.  The tensor pipe is busy 56 % of the
 // cycles, the special-function unit 43 %, the issue slots 43 %: what bounds the loop is the chain scores -> maximum -> weights
 // -> product of a row tile (about 3400 cycles a KV tile, of which the products are 1000), of which two run against each other.
 // Tried and slower: half a row per thread with sixteen softmax warps (563 us), KV tiles in halves with two score buffers (517),
@@ -33,7 +34,7 @@ constexpr int kChunkThreads = 384;  // three warpgroups; warps 10 and 11 only fi
 constexpr int kSoftmaxRegs = 224, kOtherRegs = 56;
 constexpr int kSlabBytes = 128 * 128;  // 128 rows of 64 16-bit elements, 128-byte swizzle
 constexpr float kLazyRescale = 8.0f;   // log2 of how far a weight may exceed one
-constexpr int kJoinAtOnce = 8;         // parts of an item that are joined in one step
+constexpr int kJoinAtOnce = 8;         // parts of an item that are joined in one step; 32 rows over 60000 keys, all at once 101 us, so 37
 
 template <int D>
 struct ChunkCfg {
@@ -686,7 +687,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 };
                 tc_fence_after_sync();
                 bool write = first == final;
-                if (write) {
+                if (row0 >= rows) {  // none of the warp's rows is there
+                    write = false;
+                    if (shared) b_done();
+                } else if (write) {
                     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
                     for (int c = 0; c < D / 32; ++c) {
@@ -736,18 +740,30 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     auto join = [&](int from, int step, int n, float &top, float &sum, auto &&sink) {
                         top = -INFINITY;
                         sum = 0.0f;
-#pragma unroll 8
-                        for (int i = 0; i < n; ++i) top = fmaxf(top, __ldcg(slot_of(from + i * step) + 32 * D + lane));
+                        for (int h = 0; h < n; h += 8) {  // eight loads on the way; behind the last part, it once more
+                            float m8[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) m8[i] = __ldcg(slot_of(from + min(h + i, n - 1) * step) + 32 * D + lane);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) top = fmaxf(top, m8[i]);
+                        }
                         const float ref = top == -INFINITY ? 0.0f : top;
-#pragma unroll 4
-                        for (int i = 0; i < n; ++i) {
-                            const float *pc = slot_of(from + i * step) + 32 * D + lane;
-                            sum = fmaf(__ldcg(pc + 32), fast_ex2((__ldcg(pc) - ref) * a.scale_log2), sum);
+                        for (int h = 0; h < n; h += 8) {
+                            float m8[8], l8[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const float *pc = slot_of(from + min(h + i, n - 1) * step) + 32 * D + lane;
+                                m8[i] = __ldcg(pc);
+                                l8[i] = __ldcg(pc + 32);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                if (h + i < n) sum = fmaf(l8[i], fast_ex2((m8[i] - ref) * a.scale_log2), sum);
                         }
 #pragma unroll 1
                         for (int c = 0; c < D / 32; ++c) {
                             float v[32] = {};
-#pragma unroll 2
+#pragma unroll 3
                             for (int i = 0; i < n; ++i) {
                                 const float *pc = slot_of(from + i * step);
                                 const float g = fast_ex2((__ldcg(pc + 32 * D + lane) - ref) * a.scale_log2);
