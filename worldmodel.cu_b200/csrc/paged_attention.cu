@@ -196,7 +196,9 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attention_rows_kernel(const A
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 const float mn = fmaxf(m[r], top);
                 const float ref = mn == -INFINITY ? 0.0f : mn * a.scale_log2;
-                const float corr = m[r] == -INFINITY ? 0.0f : exp2f(m[r] * a.scale_log2 - ref);
+                // of the difference, which is exactly 0 while the maximum stays: a rounded product on one side of a subtraction would
+                // multiply the sums by the same number other than one in every step
+                const float corr = m[r] == -INFINITY ? 0.0f : exp2f((m[r] - mn) * a.scale_log2);
                 m[r] = mn;
                 float sum = 0.0f;
 #pragma unroll
@@ -256,12 +258,11 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attention_rows_kernel(const A
             float top = -INFINITY;
 #pragma unroll
             for (int w = 0; w < 4; ++w) top = fmaxf(top, warp_max[w][r]);
-            const float ref = top == -INFINITY ? 0.0f : top * a.scale_log2;
             float sum = 0.0f;
             float2 v = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                const float f = warp_max[w][r] == -INFINITY ? 0.0f : exp2f(warp_max[w][r] * a.scale_log2 - ref);
+                const float f = warp_max[w][r] == -INFINITY ? 0.0f : exp2f((warp_max[w][r] - top) * a.scale_log2);
                 const float2 u = *reinterpret_cast<const float2 *>(acc + (w * kRowTile + r) * D + col);
                 sum = fmaf(warp_sum[w][r], f, sum);
                 v.x = fmaf(u.x, f, v.x);
