@@ -393,7 +393,8 @@ int b200_w8a8_kv_append(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batc
  *   causal_block = F > 0: keys up to the end of p's block of F positions, j < (p / F + 1) * F (1: plain causal; the tokens
  *                         of a frame: every frame sees itself and what came before);
  *   window = W > 0 (needs causal_block): of those, j >= (p / F + 1) * F - W, the last W up to the end of the block.
- * A token that sees no key gets zeros.  Keys and values behind a sequence's length may hold anything; what stands within
+ * A token that sees no key, or all of whose scores are minus infinity, gets zeros; a NaN or a plus infinity among the scores
+ * makes its output NaN.  Keys and values behind a sequence's length may hold anything; a value that stands within
  * the length and is hidden from a token counts with weight zero, so a NaN or infinity there spreads as zero times it.
  * q and out have the cache's type, strides in elements (multiples of 8) and 16-byte aligned pointers; they may not overlap.
  * Scores, softmax and sums are fp32; weights are rounded to the cache's type for the product with the values.

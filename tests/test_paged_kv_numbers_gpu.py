@@ -1,5 +1,7 @@
 """Attention over the paged cache at the ends of its numbers: long runs of one CTA, weights far below the largest, values that
 are no numbers, scales and head groups away from the usual ones, and how long a wait lasts."""
+import math
+
 import pytest
 import torch
 
@@ -58,3 +60,69 @@ def test_a_long_run_of_one_cta_weighs_old_and_new_keys_alike(pkg, hint):
     print("largest errors", float(off[0].max()), float(off[1].max()))
     assert bool((off[0] <= bound).all()), float(off[0].max())
     assert bool((off[1] <= bound + 2.0 ** -11).all()), float(off[1].max())
+
+
+# ------------------------------------------------------------------ no numbers
+def formula(q, k, v, mask, scale):
+    """softmax in 64 bits as torch has it, over the keys that a token sees; a token none of whose scores is above minus
+    infinity gets zeros.  q [n, heads, d], k, v [keys, kv_heads, d]."""
+    group = q.shape[1] // k.shape[1]
+    q, k, v = (x.double() for x in (q, k.repeat_interleave(group, 1), v.repeat_interleave(group, 1)))
+    s = (torch.einsum("nhd,khd->nhk", q, k) * scale).masked_fill(~mask.to(q.device)[:, None], -math.inf)
+    nothing = (s == -math.inf).all(-1, keepdim=True)
+    w = torch.where(nothing, torch.zeros_like(s), torch.softmax(s, -1))
+    return torch.einsum("nhk,khd->nhd", w, v)
+
+
+@pytest.mark.parametrize("dtype,d", [("f16", 64), ("bf16", 128), ("f16", 128), ("bf16", 64)])
+@pytest.mark.parametrize("new,hint", [(1, 1), (40, 1000), (200, 1000)])
+@pytest.mark.parametrize("what", ["nan key", "inf key", "nan query", "inf query", "nan value", "inf value"])
+def test_what_is_no_number_where_it_is_seen(pkg, dtype, d, new, hint, what):
+    """70 sequences, each with one element of one key, value or query that is NaN or infinite, at each place modulo 35 and more.
+    Outputs are NaN, infinite or finite where those of the definition are, and finite ones within the usual bound.  An infinite key
+    gives scores of plus infinity (no number is left) or minus infinity (a weight of zero) by the query's sign."""
+    t, seqs, heads, kv = pr.DTYPES[dtype], 70, 4, 2
+    keys = 70 + new
+    g = torch.Generator().manual_seed(d + new)
+    shapes = [(new, keys)] * seqs
+    k_pages, v_pages, table, contents = pr.make_cache(shapes, 32, kv, d, t, "heads", g, DEV, fill=0.0)
+    q = torch.randn(seqs, new, heads, d, generator=g).to(t)
+    q[q == 0] = 1.0
+    bad = math.nan if "nan" in what else math.inf
+    for s in range(seqs):
+        (k, v), place = contents[s], s
+        if "query" in what:
+            q[s, s % new, s % heads, s % d] = bad
+            continue
+        x, pool = (k, k_pages) if "key" in what else (v, v_pages)
+        x[place, s % kv, s % d] = bad
+        pool[int(table[s, place // 32]), s % kv, place % 32, s % d] = bad
+    cache = pkg.PagedKVCache(k_pages, v_pages)
+    batch = pkg.PagedBatch(table, pr.starts_of(shapes, DEV), pr.lens_of(shapes, DEV), max_new_tokens=hint)
+    got = pkg.paged_attention(q.view(-1, heads, d).to(DEV), cache, batch).view(seqs, new, heads, d)
+    assert pkg.poll_status() == 0
+    mask = pr.seen(new, keys, 1, 0)
+    for s in range(seqs):
+        k, v = contents[s]
+        want = formula(q[s], k, v, mask, d ** -0.5)
+        mine = got[s].cpu()
+        assert torch.equal(mine.isnan(), want.isnan()), (s, "NaN")
+        assert torch.equal(mine.isinf(), want.isinf()), (s, "infinite")
+        assert torch.equal(mine[mine.isinf()].double(), want[want.isinf()]), (s, "sign")
+        clean = [x.nan_to_num(0.0, 0.0, 0.0) for x in (q[s], k, v)]
+        _, bound = pr.attention(*clean, mask, d ** -0.5, t)
+        ok = want.isfinite()
+        assert bool(((mine.double() - want).abs() <= 2 * bound)[ok].all()), s
+
+
+def test_no_score_above_minus_infinity_gives_zeros(pkg):
+    d, kv, t = 64, 1, torch.float16
+    k = torch.zeros(50, kv, d, dtype=t, device=DEV)
+    k[:, :, 0] = -math.inf
+    v = torch.ones(50, kv, d, dtype=t, device=DEV)
+    k_pages, v_pages, table = shared_pages(k, v, 16, 1)
+    for new, hint in ((1, 1), (30, 1000)):
+        batch = pkg.PagedBatch(table, torch.tensor([0, new], dtype=torch.int32, device=DEV),
+                               torch.tensor([50], dtype=torch.int32, device=DEV), max_new_tokens=hint)
+        q = torch.ones(new, 2, d, dtype=t, device=DEV)
+        assert bool((pkg.paged_attention(q, pkg.PagedKVCache(k_pages, v_pages), batch) == 0).all())

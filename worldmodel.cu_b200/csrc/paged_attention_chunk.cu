@@ -124,9 +124,10 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void *map, uint6
         : "memory");
 }
 
-// 2^x for x in [-inf, 2^22) on the multiply-add pipe: x = n + f, n the nearest integer, |f| <= 1/2; 2^f by the polynomial of
+// 2^x for x in [-inf, 127] on the multiply-add pipe: x = n + f, n the nearest integer, |f| <= 1/2; 2^f by the polynomial of
 // least relative error over that interval among those that are exact at 0 (degree 3: 1.0e-4, for weights rounded to bf16 by
-// up to 2^-9; degree 4: 2.8e-6, for fp16's 2^-12), n added to the exponent.  x <= -127, -inf too, gives exactly 0.
+// up to 2^-9; degree 4: 2.8e-6, for fp16's 2^-12), times 2^n.  x <= -126.5, -inf too, gives exactly 0, NaN gives NaN: n added
+// to the exponent as an integer would be a step less, and make a large finite number of it.
 __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -137,7 +138,8 @@ __device__ __forceinline__ void poly_ex2(uint64_t x, float &e0, float &e1) {
     float a, b;
     unpair2(x, a, b);
     x = pair2(max_nan(a, -127.0f), max_nan(b, -127.0f));
-    const float magic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer in the low bits
+    // 1.5 * 2^23 + 127: adding it rounds to an integer, and leaves n + 127, the exponent of 2^n, in the low bits
+    const float magic = 12583039.0f;
     const uint64_t one = pair2(1.0f, 1.0f), t = add2(x, pair2(magic, magic));
     const uint64_t f = fma2(add2(t, pair2(-magic, -magic)), pair2(-1.0f, -1.0f), x);
     uint64_t p;
@@ -150,11 +152,9 @@ __device__ __forceinline__ void poly_ex2(uint64_t x, float &e0, float &e1) {
         p = fma2(p, f, pair2(0.6931241750717163f, 0.6931241750717163f));
     }
     p = fma2(p, f, one);
-    float p0, p1, t0, t1;
-    unpair2(p, p0, p1);
+    float t0, t1;
     unpair2(t, t0, t1);
-    e0 = __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23));
-    e1 = __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
+    unpair2(mul2(p, pair2(__int_as_float(__float_as_int(t0) << 23), __int_as_float(__float_as_int(t1) << 23))), e0, e1);
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
