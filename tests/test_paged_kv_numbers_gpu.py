@@ -9,6 +9,7 @@ import paged_kv_reference as pr
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
+POLY = {"f16": 2.8e-6, "bf16": 1.0e-4}  # relative error of the exponentials that the chunk kernel computes as polynomials
 
 
 def shared_pages(k, v, page, seqs):
@@ -60,6 +61,37 @@ def test_a_long_run_of_one_cta_weighs_old_and_new_keys_alike(pkg, hint):
     print("largest errors", float(off[0].max()), float(off[1].max()))
     assert bool((off[0] <= bound).all()), float(off[0].max())
     assert bool((off[1] <= bound + 2.0 ** -11).all()), float(off[1].max())
+
+
+# ------------------------------------------------------------------ weights far below the largest
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hint", [1, 1000])
+def test_many_small_weights_beside_a_large_one(pkg, dtype, hint):
+    """131071 keys, one of which has a score 18 above all others: the others' weights are 1.5e-8 of the largest, and make 0.002
+    of the sum.  Their values are one, the large one's zero in even columns.  592 sequences, so that a CTA has whole ones.
+
+    Bound: half a step for each of the two roundings of normal numbers.  fp16 weights are kept 2^7 times as large at least,
+    so that one below the normal range loses 2^-25 / 2^7 of the largest: 131071 x 2^-32.  Sums: at most 8192 additions to
+    one accumulator, 2^-23 each, above and below the fraction.  Polynomial exponentials: 1.0e-4 (bf16), 2.8e-6 (fp16), likewise."""
+    seqs, keys, d, page, t = 592, 131071, 64, 128, pr.DTYPES[dtype]
+    k = torch.zeros(keys, 1, d, dtype=t, device=DEV)
+    k[777] = 2.25  # 64 x 2.25 / 8 = 18
+    v = torch.ones(keys, 1, d, dtype=t, device=DEV)
+    v[777, :, ::2] = 0.0
+    k_pages, v_pages, table = shared_pages(k, v, page, seqs)
+    q = torch.ones(seqs, 1, d, dtype=t, device=DEV)
+    batch = pkg.PagedBatch(table, torch.arange(seqs + 1, dtype=torch.int32, device=DEV),
+                           torch.full((seqs,), keys, dtype=torch.int32, device=DEV), max_new_tokens=hint)
+    got = pkg.paged_attention(q, pkg.PagedKVCache(k_pages, v_pages), batch).double()
+    small = (keys - 1) * math.exp(-18.0)
+    want = small / (1 + small)
+    lost = keys * 2.0 ** -32 if dtype == "f16" else 0.0
+    rel = 2 * pr.half_step(t) + 8192 * 2 * 2.0 ** -23 + 2 * POLY[dtype]
+    off = float((got[..., ::2] - want).abs().max()), float((got[..., 1::2] - 1).abs().max())
+    print("largest errors", off, "of", want)
+    assert pkg.poll_status() == 0
+    assert off[0] <= rel * want + lost, off
+    assert off[1] <= rel + lost, off
 
 
 # ------------------------------------------------------------------ no numbers

@@ -28,6 +28,13 @@ constexpr int kRowsKeyTile = kStepKeys * (kRowsThreads / 32);  // keys per KV ti
 // as well), one of 131071 keys 95.8 / 94.0 / 93.3 us
 constexpr int kRowsExtra = 2;
 
+// log2 of a factor that all weights carry, and that cancels: the largest is 2^15 in fp16, whose least normal number is 2^-14, so
+// that the many small weights of a long sequence beside a large one are not lost.
+template <typename T>
+constexpr float kWeightsUp = 0.0f;
+template <>
+constexpr float kWeightsUp<__half> = 15.0f;
+
 template <int D>
 struct RowsCfg {
     static constexpr int kStepBytes = 2 * kStepKeys * D * 2;  // keys and values of a step
@@ -195,7 +202,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attention_rows_kernel(const A
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 const float mn = fmaxf(m[r], top);
-                const float ref = mn == -INFINITY ? 0.0f : mn * a.scale_log2;
+                const float ref = mn == -INFINITY ? 0.0f : mn * a.scale_log2 - kWeightsUp<T>;
                 // of the difference, which is exactly 0 while the maximum stays: a rounded product on one side of a subtraction would
                 // multiply the sums by the same number other than one in every step
                 const float corr = m[r] == -INFINITY ? 0.0f : exp2f((m[r] - mn) * a.scale_log2);

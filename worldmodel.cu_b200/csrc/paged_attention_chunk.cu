@@ -6,7 +6,9 @@
 // softmax of A and of B, one thread per row, so that row maxima and sums need no exchange.  While A's weights are computed the
 // tensor core works on B.  The running maximum moves only when a row has outgrown it by 2^8 (weights stay below 2^8, and the
 // factor cancels in the quotient), so O in tensor memory is rescaled rarely.  Weights are rounded to the cache's type, half a
-// step each: that is what the tensor core takes; their sum is taken before, in fp32.
+// step each: that is what the tensor core takes; their sum is taken before, in fp32.  fp16 weights carry a factor 2^7 more, up to
+// 2^15 in all, so that those of a long sequence beside a large one stay above the least number of that type (131071 keys
+// beside one that is 2^26 times as large: without it their share of the output was lost).
 // Keys stay K-major as they lie in the page, values are read in the same layout as the MN-major operand: nothing is
 // transposed.  Rows of V outside the sequence are zeroed in shared memory before their product, since 0 x NaN is no zero.
 // An item of at most 128 rows has no second row tile: both accumulators work on it, KV tiles in turn.
@@ -34,6 +36,7 @@ constexpr int kChunkThreads = 384;  // three warpgroups; warps 10 and 11 only fi
 constexpr int kSoftmaxRegs = 224, kOtherRegs = 56;
 constexpr int kSlabBytes = 128 * 128;  // 128 rows of 64 16-bit elements, 128-byte swizzle
 constexpr float kLazyRescale = 8.0f;   // log2 of how far a weight may exceed one
+constexpr float kWeightsUp = 7.0f;     // log2 of the factor of fp16 weights
 constexpr int kJoinAtOnce = 8;         // parts of an item that are joined in one step; 32 rows over 60000 keys, all at once 101 us, so 37
 
 template <int D>
@@ -576,7 +579,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                             tmem_st_32x16(to + 16 * c, o);
                         }
                     }
-                    const float ref = m == -INFINITY ? 0.0f : m * a.scale_log2;
+                    const float ref = m == -INFINITY ? 0.0f : m * a.scale_log2 - (IsBf16<T>::value ? 0.0f : kWeightsUp);
                     const uint64_t scale2 = pair2(a.scale_log2, a.scale_log2), ref2 = pair2(-ref, -ref);
                     uint64_t sum[4] = {};
                     // weights of 32 keys at a time over the scores, which are in registers by now.  Some pairs go to the
