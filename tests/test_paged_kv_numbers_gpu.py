@@ -158,3 +158,38 @@ def test_no_score_above_minus_infinity_gives_zeros(pkg):
                                torch.tensor([50], dtype=torch.int32, device=DEV), max_new_tokens=hint)
         q = torch.ones(new, 2, d, dtype=t, device=DEV)
         assert bool((pkg.paged_attention(q, pkg.PagedKVCache(k_pages, v_pages), batch) == 0).all())
+
+
+# ------------------------------------------------------------------ waits
+@pytest.mark.parametrize("limit_ms", [20, 200])
+def test_a_wait_lasts_as_long_as_its_limit(pkg, limit_ms):
+    """One page load left out by the test switch: the kernel gives up no sooner than the limit says, and soon after it."""
+    L = pkg.lib()
+    seqs, heads, kv, d = [(300, 2000), (40, 64)], 4, 2, 64
+    g = torch.Generator().manual_seed(1)
+    k_pages, v_pages, table, _ = pr.make_cache(seqs, 32, kv, d, torch.float16, "heads", g, DEV)
+    cache = pkg.PagedKVCache(k_pages, v_pages)
+    batch = pkg.PagedBatch(table, pr.starts_of(seqs, DEV), pr.lens_of(seqs, DEV))
+    q = torch.randn(340, heads, d, generator=g).half().to(DEV)
+    ws = pkg.make_attention_workspace(cache)
+    want = pkg.paged_attention(q, cache, batch, workspace=ws)
+    torch.cuda.synchronize()
+    begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    try:
+        L.b200_w8a8_debug_set_wait_limit_ns(limit_ms * 1_000_000)
+        L.b200_w8a8_debug_drop_operand_load(1)
+        begin.record()
+        pkg.paged_attention(q, cache, batch, workspace=ws)
+        end.record()
+        torch.cuda.synchronize()
+        took = begin.elapsed_time(end)
+        with pytest.raises(pkg.W8A8Error, match="gave up a bounded wait"):
+            pkg.paged_attention(q, cache, batch, workspace=ws)
+    finally:
+        L.b200_w8a8_debug_drop_operand_load(0)
+        L.b200_w8a8_debug_set_wait_limit_ns(0)
+    print("limit", limit_ms, "ms, took", took)
+    ws.zero_()
+    assert torch.equal(pkg.paged_attention(q, cache, batch, workspace=ws), want)
+    assert pkg.poll_status() == 0
+    assert limit_ms <= took <= 4 * limit_ms + 100
