@@ -193,3 +193,16 @@ def test_a_wait_lasts_as_long_as_its_limit(pkg, limit_ms):
     assert torch.equal(pkg.paged_attention(q, cache, batch, workspace=ws), want)
     assert pkg.poll_status() == 0
     assert limit_ms <= took <= 4 * limit_ms + 100
+
+
+# ------------------------------------------------------------------ types
+@pytest.mark.parametrize("dtype", [torch.float64, torch.int64, torch.uint8, torch.float8_e4m3fn, torch.float32, torch.int32])
+def test_other_types_are_refused(pkg, dtype):
+    pages = torch.zeros(2, 1, 16, 64, device=DEV)
+    x = torch.zeros(1, 1, 64, device=DEV)
+    batch = pkg.PagedBatch(*(torch.tensor(v, dtype=torch.int32, device=DEV) for v in ([[0]], [0, 1], [1])))
+    with pytest.raises(pkg.W8A8Error):
+        pkg.kv_append(pkg.PagedKVCache(pages.to(dtype), pages.to(dtype)), batch, x, x)
+    if dtype != torch.float32:
+        with pytest.raises(pkg.W8A8Error):
+            pkg.kv_append(pkg.PagedKVCache(pages.half(), pages.half()), batch, x.to(dtype), x.to(dtype))

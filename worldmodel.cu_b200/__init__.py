@@ -156,7 +156,10 @@ def _dt(t) -> int:
     if not _dt_codes:
         import torch
         _dt_codes.update({torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16, torch.int32: DT_S32})
-    return _dt_codes[t.dtype]
+    code = _dt_codes.get(t.dtype)
+    if code is None:
+        raise W8A8Error(f"no operator takes tensors of type {t.dtype}")
+    return code
 
 
 def mma_rate(slabs_per_cta=16384) -> float:
