@@ -160,6 +160,25 @@ def test_no_score_above_minus_infinity_gives_zeros(pkg):
         assert bool((pkg.paged_attention(q, pkg.PagedKVCache(k_pages, v_pages), batch) == 0).all())
 
 
+# ------------------------------------------------------------------ workspaces
+@pytest.mark.parametrize("new,keys", [(1, 40000), (32, 60000), (300, 9000)])
+def test_of_a_workspace_only_the_counters_have_to_be_zero(pkg, new, keys):
+    heads, kv, d = 4, 1, 64
+    g = torch.Generator().manual_seed(new)
+    k_pages, v_pages, table, _ = pr.make_cache([(new, keys)], 64, kv, d, torch.float16, "heads", g, DEV, fill=0.0)
+    cache = pkg.PagedKVCache(k_pages, v_pages)
+    batch = pkg.PagedBatch(table, pr.starts_of([(new, keys)], DEV), pr.lens_of([(new, keys)], DEV), max_new_tokens=new)
+    q = torch.randn(new, heads, d, generator=g).half().to(DEV)
+    clean = pkg.make_attention_workspace(cache)
+    clean.zero_()
+    dirty = torch.full_like(clean, 255)  # NaN as floats
+    dirty[:32768] = 0
+    want = pkg.paged_attention(q, cache, batch, workspace=clean)
+    assert torch.equal(pkg.paged_attention(q, cache, batch, workspace=dirty), want) and bool(want.isfinite().all())
+    assert torch.equal(pkg.paged_attention(q, cache, batch), want)
+    assert pkg.poll_status() == 0
+
+
 # ------------------------------------------------------------------ waits
 @pytest.mark.parametrize("limit_ms", [20, 200])
 def test_a_wait_lasts_as_long_as_its_limit(pkg, limit_ms):

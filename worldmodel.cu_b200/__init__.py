@@ -605,12 +605,14 @@ def kv_append(cache, batch, k, v, q=None, q_out=None, norm_eps=None, q_weight=No
 
 
 def make_attention_workspace(cache):
-    """Zero-filled scratch for paged_attention over caches of this head size on this device.  Every call leaves its
-    counters zero, so one buffer serves all calls that do not overlap on the GPU."""
+    """Scratch for paged_attention over caches of this head size on this device, its counters zero.  Every call leaves them
+    zero, so one buffer serves all calls that do not overlap on the GPU."""
     import torch
     with torch.cuda.device(cache.index):
         nbytes = lib().b200_w8a8_paged_attention_workspace_size(cache.d_head)
-        return torch.zeros(nbytes, dtype=torch.uint8, device=cache.k_pages.device)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=cache.k_pages.device)
+        workspace[:32768].zero_()  # the counters; the rest, up to 39 MB, is written before it is read
+        return workspace
 
 
 def paged_attention(q, cache, batch, scale=None, causal_block=1, window=0, out=None, workspace=None):
