@@ -160,6 +160,49 @@ def test_no_score_above_minus_infinity_gives_zeros(pkg):
         assert bool((pkg.paged_attention(q, pkg.PagedKVCache(k_pages, v_pages), batch) == 0).all())
 
 
+# ------------------------------------------------------------------ scales and head groups
+def definition(q, k, v, n, keys, scale, dtype):
+    """The output in 64 bits and its bound, the polynomials' term among it: an error of that size in every weight, in
+    numerator and denominator."""
+    t, mask = pr.DTYPES[dtype], pr.seen(n, keys, 1, 0)
+    want, bound = pr.attention(q, k.to(DEV), v.to(DEV), mask, scale, t)
+    return want, bound + 2 * POLY[dtype] * pr.attention(q, k.to(DEV), v.abs().to(DEV), mask, scale, t)[0]
+
+
+@pytest.mark.parametrize("scale", [1.0, 0.3, 1e-4, 3.0])
+@pytest.mark.parametrize("dtype,d", [("f16", 64), ("bf16", 128)])
+def test_scales(pkg, scale, dtype, d):
+    t, heads, kv, shapes = pr.DTYPES[dtype], 6, 2, [(1, 300), (90, 400), (1, 1), (9, 2000)]
+    g = torch.Generator().manual_seed(d)
+    k_pages, v_pages, table, contents = pr.make_cache(shapes, 32, kv, d, t, "heads", g, DEV)
+    cache, starts = pkg.PagedKVCache(k_pages, v_pages), pr.starts_of(shapes, DEV)
+    q = torch.randn(101, heads, d, generator=g).to(t).to(DEV)
+    for hint in (1, 1000):
+        out = pkg.paged_attention(q, cache, pkg.PagedBatch(table, starts, pr.lens_of(shapes, DEV), max_new_tokens=hint), scale=scale)
+        at = 0
+        for (n, keys), (k, v) in zip(shapes, contents):
+            want, bound = definition(q[at:at + n], k, v, n, keys, scale, dtype)
+            assert bool(((out[at:at + n].double() - want).abs() <= bound).all()), (hint, n, keys)
+            at += n
+    assert pkg.poll_status() == 0
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (9, 3), (5, 1), (14, 2), (16, 1), (40, 2), (48, 1)])
+@pytest.mark.parametrize("new", [1, 3, 37])
+@pytest.mark.parametrize("dtype,d,order", [("bf16", 128, "tokens"), ("f16", 128, "heads"), ("bf16", 64, "heads")])
+def test_head_groups_of_every_kernel(pkg, heads, kv_heads, new, dtype, d, order):
+    t, shapes = pr.DTYPES[dtype], [(new, 200), (new, new), (new, 77)]
+    g = torch.Generator().manual_seed(heads)
+    k_pages, v_pages, table, contents = pr.make_cache(shapes, 64, kv_heads, d, t, order, g, DEV)
+    q = torch.randn(3 * new, heads, d, generator=g).to(t).to(DEV)
+    batch = pkg.PagedBatch(table, pr.starts_of(shapes, DEV), pr.lens_of(shapes, DEV), max_new_tokens=new)
+    out = pkg.paged_attention(q, pkg.PagedKVCache(k_pages, v_pages), batch)
+    assert pkg.poll_status() == 0
+    for i, ((n, keys), (k, v)) in enumerate(zip(shapes, contents)):
+        want, bound = definition(q[i * new:(i + 1) * new], k, v, n, keys, d ** -0.5, dtype)
+        assert bool(((out[i * new:(i + 1) * new].double() - want).abs() <= bound).all()), (n, keys)
+
+
 # ------------------------------------------------------------------ workspaces
 @pytest.mark.parametrize("new,keys", [(1, 40000), (32, 60000), (300, 9000)])
 def test_of_a_workspace_only_the_counters_have_to_be_zero(pkg, new, keys):
