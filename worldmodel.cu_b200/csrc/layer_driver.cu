@@ -186,6 +186,7 @@ int b200_w8a8_layer_forward_paged(void *handle, const b200_w8a8_layer *L, const 
     if (check_controller(L, "layer_forward_paged")) return 1;
     const int T = batch->n_tokens, d = c->d, dh = c->d_head;
     if (T <= 0 || T > c->max_tokens) return fail("layer_forward_paged: %d tokens, the context holds %d", T, c->max_tokens);
+    if (batch->n_seqs <= 0) return fail("layer_forward_paged: %d tokens of %d sequences", T, batch->n_seqs);
     if (cache->n_kv_heads != c->n_kv_heads || cache->d_head != dh)
         return fail("layer_forward_paged: the cache has %d heads of %d, the layer %d of %d", cache->n_kv_heads, cache->d_head,
                     c->n_kv_heads, dh);
