@@ -89,11 +89,11 @@ int status_check_entry() {
     *h = 0;
     gemm_reset_static_tickets();
     if (code == KS_BAD_PAGE)
-        return fail("an earlier append or attention met a sequence length or page index outside its cache, or row "
-                    "starts that overlap (status %d); "
+        return fail("an earlier append or attention met a sequence length or page index outside its cache, a position "
+                    "outside its rotation tables, or row starts that overlap (status %d); "
                     "nothing was accessed there and the results of that sequence are undefined", code);
     return fail("an earlier kernel gave up a bounded wait (status %d: %s); the outputs of that launch are incomplete, "
-                "and a split-K workspace it used must be zeroed again before reuse",
+                "and a split-K workspace or the counters of an attention workspace that it used must be zeroed again before reuse",
                 code, status_text(code));
 }
 
