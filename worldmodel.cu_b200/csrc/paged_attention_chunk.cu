@@ -227,7 +227,8 @@ struct ChunkExtra {
     int debug_drop_load;
 };
 
-// An item of one row tile: both accumulators work on it, KV tiles in turn, and are joined at the end of a run.
+// An item of one row tile: both accumulators work on it, KV tiles in turn, and are joined at the end of a run.  Of other items
+// both row tiles hold rows.
 __device__ __forceinline__ bool is_shared(const Item &it) { return it.rows - it.rt * kChunkRows <= 128; }
 
 template <typename T, int D>
@@ -499,125 +500,122 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             const int kt0 = now.kt0, kt1 = now.kt1;
             const bool shared = is_shared(it);
             const int row0 = it.rt * kChunkRows + (shared ? 0 : tile * 128) + sub * 32;
-            const bool active = shared || it.rt * kChunkRows + tile * 128 < it.rows;
             const int kt_first = shared ? kt0 + tile : kt0, kt_step = shared ? 2 : 1;
             float m = -INFINITY, l = 0.0f;
             const int item_lo = it.lo, item_hi = it.hi;
-            if (active) {
-                if (first_run && (tile == 0 || !shared)) load_q(row0);
-                int lo = 0, hi = 0x7fffffff;  // a row that is not there masks nothing
-                if (row0 + lane < it.rows)
-                    visible_keys(a, it.seq.keys - it.seq.n + a.by_group.div(row0 + lane), it.seq.keys, lo, hi);
-                const int lo_max = __reduce_max_sync(0xffffffffu, lo), hi_min = __reduce_min_sync(0xffffffffu, hi);
-                for (int kt = kt_first; kt < kt1; kt += kt_step) {
-                    ok = wait_bounded(s_full + 8 * tile, s_ph, abort_flag, ex.wait_limit, KS_TIMEOUT_SOFTMAX);
-                    ok = __all_sync(0xffffffffu, ok);
+            if (first_run && (tile == 0 || !shared)) load_q(row0);
+            int lo = 0, hi = 0x7fffffff;  // a row that is not there masks nothing
+            if (row0 + lane < it.rows)
+                visible_keys(a, it.seq.keys - it.seq.n + a.by_group.div(row0 + lane), it.seq.keys, lo, hi);
+            const int lo_max = __reduce_max_sync(0xffffffffu, lo), hi_min = __reduce_min_sync(0xffffffffu, hi);
+            for (int kt = kt_first; kt < kt1; kt += kt_step) {
+                ok = wait_bounded(s_full + 8 * tile, s_ph, abort_flag, ex.wait_limit, KS_TIMEOUT_SOFTMAX);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                s_ph ^= 1u;
+                tc_fence_after_sync();
+                // Values of keys that the item's rows do not see may be anything, NaN too, and 0 x NaN is no zero: the four
+                // warps whose product comes first clear them before their weights let it begin
+                if ((tile == 0 || shared) && (kt * kKeyTile < item_lo || (kt + 1) * kKeyTile > item_hi)) {
+                    const unsigned at = 2u * (unsigned)(tiles_before + kt - kt0) + 1u, stage = at % C::kStages;
+                    ok = __all_sync(0xffffffffu, wait_bounded(kv_full + 8 * stage, at / C::kStages & 1u, abort_flag,
+                                                              ex.wait_limit, KS_TIMEOUT_SMEM_FULL));
                     if (!ok) break;
-                    s_ph ^= 1u;
-                    tc_fence_after_sync();
-                    // Values of keys that the item's rows do not see may be anything, NaN too, and 0 x NaN is no zero: the four
-                    // warps whose product comes first clear them before their weights let it begin
-                    if ((tile == 0 || shared) && (kt * kKeyTile < item_lo || (kt + 1) * kKeyTile > item_hi)) {
-                        const unsigned at = 2u * (unsigned)(tiles_before + kt - kt0) + 1u, stage = at % C::kStages;
-                        ok = __all_sync(0xffffffffu, wait_bounded(kv_full + 8 * stage, at / C::kStages & 1u, abort_flag,
-                                                                  ex.wait_limit, KS_TIMEOUT_SMEM_FULL));
-                        if (!ok) break;
-                        uint8_t *v = ring + stage * C::kTileBytes;
-                        for (int row = sub * 32 + lane / 8; row < sub * 32 + 32; row += 4) {
-                            const int key = kt * kKeyTile + row;
-                            if (key < item_lo || key >= item_hi) {
+                    uint8_t *v = ring + stage * C::kTileBytes;
+                    for (int row = sub * 32 + lane / 8; row < sub * 32 + 32; row += 4) {
+                        const int key = kt * kKeyTile + row;
+                        if (key < item_lo || key >= item_hi) {
 #pragma unroll
-                                for (int d = 0; d < D / 64; ++d)
-                                    *reinterpret_cast<uint4 *>(v + d * kSlabBytes + row * 128 + (lane & 7) * 16) =
-                                        make_uint4(0, 0, 0, 0);
-                            }
-                        }
-                        fence_proxy_async_smem();
-                    }
-                    uint32_t s[4][32];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_ld_32x32(ts + 32 * c, s[c]);
-                    tmem_ld_wait();
-                    auto f = [&](int i) { return __uint_as_float(s[i / 32][i % 32]); };
-                    const int key0 = kt * kKeyTile;
-                    if (key0 < lo_max || key0 + kKeyTile > hi_min) {
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const int from = lo - key0 - 32 * c, upto = hi - key0 - 32 * c;
-                            if (lo_max > key0 + 32 * c) {
-#pragma unroll
-                                for (int i = 0; i < 32; ++i)
-                                    if (i < from) s[c][i] = 0xff800000u;
-                            }
-                            if (hi_min < key0 + 32 * c + 32) {
-#pragma unroll
-                                for (int i = 0; i < 32; ++i)
-                                    if (i >= upto) s[c][i] = 0xff800000u;
-                            }
+                            for (int d = 0; d < D / 64; ++d)
+                                *reinterpret_cast<uint4 *>(v + d * kSlabBytes + row * 128 + (lane & 7) * 16) =
+                                    make_uint4(0, 0, 0, 0);
                         }
                     }
-                    float t8[8];
+                    fence_proxy_async_smem();
+                }
+                uint32_t s[4][32];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        t8[i] = f(i);
-#pragma unroll
-                        for (int j = 8; j < kKeyTile - 8; j += 16) t8[i] = max3(t8[i], f(i + j), f(i + j + 8));
-                        t8[i] = fmaxf(t8[i], f(i + kKeyTile - 8));
-                    }
-                    const float top = max3(max3(t8[0], t8[1], t8[2]), max3(t8[3], t8[4], t8[5]), fmaxf(t8[6], t8[7]));
-                    if (kt == kt_first) {
-                        m = top;
-                    } else if (__any_sync(0xffffffffu, (top - m) * a.scale_log2 > kLazyRescale)) {
-                        const float mn = fmaxf(m, top);
-                        const float g = m == -INFINITY ? 0.0f : fast_ex2((m - mn) * a.scale_log2);
-                        m = mn;
-                        l *= g;
-#pragma unroll
-                        for (int c = 0; c < D / 16; ++c) {
-                            uint32_t o[16];
-                            tmem_ld_32x16(to + 16 * c, o);
-                            tmem_ld_wait();
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * g);
-                            tmem_st_32x16(to + 16 * c, o);
-                        }
-                    }
-                    const float ref = m == -INFINITY ? 0.0f : m * a.scale_log2 - (IsBf16<T>::value ? 0.0f : kWeightsUp);
-                    const uint64_t scale2 = pair2(a.scale_log2, a.scale_log2), ref2 = pair2(-ref, -ref);
-                    uint64_t sum[4] = {};
-                    // weights of 32 keys at a time over the scores, which are in registers by now.  Some pairs go to the
-                    // multiply-add pipe, the others to the special-function unit, which alone would bound the kernel.
+                for (int c = 0; c < 4; ++c) tmem_ld_32x32(ts + 32 * c, s[c]);
+                tmem_ld_wait();
+                auto f = [&](int i) { return __uint_as_float(s[i / 32][i % 32]); };
+                const int key0 = kt * kKeyTile;
+                if (key0 < lo_max || key0 + kKeyTile > hi_min) {
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        uint32_t w[16];
+                        const int from = lo - key0 - 32 * c, upto = hi - key0 - 32 * c;
+                        if (lo_max > key0 + 32 * c) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const uint64_t v = fma2(pair2(f(32 * c + 2 * i), f(32 * c + 2 * i + 1)), scale2, ref2);
-                            float e0, e1;
-                            if ((i & 7) < kPolyPairs<D>) {
-                                poly_ex2<IsBf16<T>::value ? 3 : 4>(v, e0, e1);
-                            } else {
-                                unpair2(v, e0, e1);
-                                e0 = fast_ex2(e0);
-                                e1 = fast_ex2(e1);
-                            }
-                            sum[i & 3] = add2(sum[i & 3], pair2(e0, e1));
-                            w[i] = Half2Of<T>::pack(e0, e1);
+                            for (int i = 0; i < 32; ++i)
+                                if (i < from) s[c][i] = 0xff800000u;
                         }
-                        tmem_st_32x16(ts + 16 * c, w);
-                        if (c & 1) {  // half of the weights: their product may begin
-                            tmem_st_wait();
-                            tc_fence_before_sync();
-                            __syncwarp();
-                            if (lane == 0) arrive_on(p_ready + 16 * tile + 8 * (c / 2));
+                        if (hi_min < key0 + 32 * c + 32) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (i >= upto) s[c][i] = 0xff800000u;
                         }
                     }
-                    float l0, l1;
-                    unpair2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), l0, l1);
-                    l += l0 + l1;
                 }
-                if (!ok) break;
+                float t8[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    t8[i] = f(i);
+#pragma unroll
+                    for (int j = 8; j < kKeyTile - 8; j += 16) t8[i] = max3(t8[i], f(i + j), f(i + j + 8));
+                    t8[i] = fmaxf(t8[i], f(i + kKeyTile - 8));
+                }
+                const float top = max3(max3(t8[0], t8[1], t8[2]), max3(t8[3], t8[4], t8[5]), fmaxf(t8[6], t8[7]));
+                if (kt == kt_first) {
+                    m = top;
+                } else if (__any_sync(0xffffffffu, (top - m) * a.scale_log2 > kLazyRescale)) {
+                    const float mn = fmaxf(m, top);
+                    const float g = m == -INFINITY ? 0.0f : fast_ex2((m - mn) * a.scale_log2);
+                    m = mn;
+                    l *= g;
+#pragma unroll
+                    for (int c = 0; c < D / 16; ++c) {
+                        uint32_t o[16];
+                        tmem_ld_32x16(to + 16 * c, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * g);
+                        tmem_st_32x16(to + 16 * c, o);
+                    }
+                }
+                const float ref = m == -INFINITY ? 0.0f : m * a.scale_log2 - (IsBf16<T>::value ? 0.0f : kWeightsUp);
+                const uint64_t scale2 = pair2(a.scale_log2, a.scale_log2), ref2 = pair2(-ref, -ref);
+                uint64_t sum[4] = {};
+                // weights of 32 keys at a time over the scores, which are in registers by now.  Some pairs go to the
+                // multiply-add pipe, the others to the special-function unit, which alone would bound the kernel.
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const uint64_t v = fma2(pair2(f(32 * c + 2 * i), f(32 * c + 2 * i + 1)), scale2, ref2);
+                        float e0, e1;
+                        if ((i & 7) < kPolyPairs<D>) {
+                            poly_ex2<IsBf16<T>::value ? 3 : 4>(v, e0, e1);
+                        } else {
+                            unpair2(v, e0, e1);
+                            e0 = fast_ex2(e0);
+                            e1 = fast_ex2(e1);
+                        }
+                        sum[i & 3] = add2(sum[i & 3], pair2(e0, e1));
+                        w[i] = Half2Of<T>::pack(e0, e1);
+                    }
+                    tmem_st_32x16(ts + 16 * c, w);
+                    if (c & 1) {  // half of the weights: their product may begin
+                        tmem_st_wait();
+                        tc_fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) arrive_on(p_ready + 16 * tile + 8 * (c / 2));
+                    }
+                }
+                float l0, l1;
+                unpair2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), l0, l1);
+                l += l0 + l1;
             }
+            if (!ok) break;
             // what the end of this run needs, then on to the next item, whose queries come to L2 meanwhile
             tiles_before += kt1 - kt0;
             const int first = now.first, final = now.final, rows = it.rows, head0 = it.h * a.group, q0 = it.seq.q0;
@@ -631,217 +629,215 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 }
             }
             first_run = false;
-            if (active) {
-                const bool mine_any = kt_first < kt1;  // B has nothing in a run of one KV tile
-                if (shared && tile == 1) {
-                    float *stats = const_cast<float *>(b_stats);
-                    stats[lane] = m;
-                    stats[32 + lane] = l;
-                    __syncwarp();
-                    if (lane == 0) arrive_on(b_known + 8 * sub);
-                    ok = wait_bounded(b_taken + 8 * sub, known_ph, abort_flag, ex.wait_limit, KS_TIMEOUT_TMEM_FULL);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    known_ph ^= 1u;
-                    if (mine_any) o_ph ^= 1u;
-                    if (more) load_q(it.rt * kChunkRows + tile * 128 + sub * 32);
-                    continue;
-                }
-                ok = wait_bounded(o_full + 8 * tile, o_ph, abort_flag, ex.wait_limit, KS_TIMEOUT_TMEM_FULL);
+            const bool mine_any = kt_first < kt1;  // B has nothing in a run of one KV tile
+            if (shared && tile == 1) {
+                float *stats = const_cast<float *>(b_stats);
+                stats[lane] = m;
+                stats[32 + lane] = l;
+                __syncwarp();
+                if (lane == 0) arrive_on(b_known + 8 * sub);
+                ok = wait_bounded(b_taken + 8 * sub, known_ph, abort_flag, ex.wait_limit, KS_TIMEOUT_TMEM_FULL);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                o_ph ^= 1u;
-                // this row's factors of the two accumulators
-                float fa = 1.0f, fb = 0.0f;
-                if (shared) {
-                    const bool b_any = kt0 + 1 < kt1;
-                    ok = wait_bounded(b_known + 8 * sub, known_ph, abort_flag, ex.wait_limit, KS_TIMEOUT_TMEM_FULL);
-                    if (ok && b_any) ok = wait_bounded(o_full + 8, b_ph, abort_flag, ex.wait_limit, KS_TIMEOUT_TMEM_FULL);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    known_ph ^= 1u;
-                    if (b_any) {
-                        b_ph ^= 1u;
-                        const float mb = b_stats[lane], lb = b_stats[32 + lane], top = fmaxf(m, mb);
-                        const float ref = top == -INFINITY ? 0.0f : top;
-                        fa = fast_ex2((m - ref) * a.scale_log2);
-                        fb = fast_ex2((mb - ref) * a.scale_log2);
-                        m = top;
-                        l = l * fa + lb * fb;
-                    }
-                } else {
+                known_ph ^= 1u;
+                if (mine_any) o_ph ^= 1u;
+                if (more) load_q(it.rt * kChunkRows + tile * 128 + sub * 32);
+                continue;
+            }
+            ok = wait_bounded(o_full + 8 * tile, o_ph, abort_flag, ex.wait_limit, KS_TIMEOUT_TMEM_FULL);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            o_ph ^= 1u;
+            // this row's factors of the two accumulators
+            float fa = 1.0f, fb = 0.0f;
+            if (shared) {
+                const bool b_any = kt0 + 1 < kt1;
+                ok = wait_bounded(b_known + 8 * sub, known_ph, abort_flag, ex.wait_limit, KS_TIMEOUT_TMEM_FULL);
+                if (ok && b_any) ok = wait_bounded(o_full + 8, b_ph, abort_flag, ex.wait_limit, KS_TIMEOUT_TMEM_FULL);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                known_ph ^= 1u;
+                if (b_any) {
                     b_ph ^= 1u;
+                    const float mb = b_stats[lane], lb = b_stats[32 + lane], top = fmaxf(m, mb);
+                    const float ref = top == -INFINITY ? 0.0f : top;
+                    fa = fast_ex2((m - ref) * a.scale_log2);
+                    fb = fast_ex2((mb - ref) * a.scale_log2);
+                    m = top;
+                    l = l * fa + lb * fb;
                 }
-                const bool two = shared && kt0 + 1 < kt1;
-                auto b_done = [&]() {  // B may go on to its next run
-                    tc_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) arrive_on(b_taken + 8 * sub);
-                };
-                auto load_o = [&](int c, float (&o)[32]) {  // columns 32 c .. of this row's sum
-                    uint32_t u[32];
-                    tmem_ld_32x32(to + 32 * c, u);
+            } else {
+                b_ph ^= 1u;
+            }
+            const bool two = shared && kt0 + 1 < kt1;
+            auto b_done = [&]() {  // B may go on to its next run
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) arrive_on(b_taken + 8 * sub);
+            };
+            auto load_o = [&](int c, float (&o)[32]) {  // columns 32 c .. of this row's sum
+                uint32_t u[32];
+                tmem_ld_32x32(to + 32 * c, u);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(u[i]);
+                if (two) {
+                    tmem_ld_32x32(to + D + 32 * c, u);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(u[i]);
-                    if (two) {
-                        tmem_ld_32x32(to + D + 32 * c, u);
-                        tmem_ld_wait();
+                    for (int i = 0; i < 32; ++i) o[i] = fmaf(__uint_as_float(u[i]), fb, o[i] * fa);
+                }
+            };
+            tc_fence_after_sync();
+            bool write = first == final;
+            if (row0 >= rows) {  // none of the warp's rows is there
+                write = false;
+                if (shared) b_done();
+            } else if (write) {
+                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = fmaf(__uint_as_float(u[i]), fb, o[i] * fa);
+                for (int c = 0; c < D / 32; ++c) {
+                    float o[32];
+                    load_o(c, o);
+                    auto g = [&](int i) { return o[i] * inv; };
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        *reinterpret_cast<uint4 *>(chunk_at(lane, 4 * c + i)) =
+                            make_uint4(Half2Of<T>::pack(g(8 * i), g(8 * i + 1)), Half2Of<T>::pack(g(8 * i + 2), g(8 * i + 3)),
+                                       Half2Of<T>::pack(g(8 * i + 4), g(8 * i + 5)), Half2Of<T>::pack(g(8 * i + 6), g(8 * i + 7)));
+                }
+                if (shared) b_done();
+            } else {
+                // [slot of the CTA][warp]: columns in vectors of four, 32 rows each
+                const int parts = final - first + 1;
+                auto slot_of = [&](int cta) {
+                    return a.partials + ((long long)(2 * cta + (cta == first ? 1 : 0)) * 8 + warp) * C::kWarpPartial;
+                };
+                float *part = slot_of((int)blockIdx.x);
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    float o[32];
+                    load_o(c, o);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        *reinterpret_cast<float4 *>(part + ((8 * c + i) * 32 + lane) * 4) =
+                            make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                }
+                if (shared) b_done();
+                part[32 * D + lane] = m;
+                part[32 * D + 32 + lane] = l;
+                // whether this warp is the last of n to arrive at a counter; then the others' parts can be read
+                auto last_of = [&](int *ticket, int n) {
+                    __threadfence();
+                    __syncwarp();
+                    int before = 0;
+                    if (lane == 0) {
+                        before = atomicAdd(ticket, 1);
+                        if (before == n - 1) *ticket = 0;  // zero again for the next launch
+                    }
+                    before = __shfl_sync(0xffffffffu, before, 0);
+                    __threadfence();
+                    return before == n - 1;
+                };
+                // joins parts of the CTAs from, from + step, ...: maximum and sum, then 32 columns at a time to `sink`
+                auto join = [&](int from, int step, int n, float &top, float &sum, auto &&sink) {
+                    top = -INFINITY;
+                    sum = 0.0f;
+                    for (int h = 0; h < n; h += 8) {  // eight loads on the way; behind the last part, it once more
+                        float m8[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) m8[i] = __ldcg(slot_of(from + min(h + i, n - 1) * step) + 32 * D + lane);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) top = fmaxf(top, m8[i]);
+                    }
+                    const float ref = top == -INFINITY ? 0.0f : top;
+                    for (int h = 0; h < n; h += 8) {
+                        float m8[8], l8[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float *pc = slot_of(from + min(h + i, n - 1) * step) + 32 * D + lane;
+                            m8[i] = __ldcg(pc);
+                            l8[i] = __ldcg(pc + 32);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (h + i < n) sum = fmaf(l8[i], fast_ex2((m8[i] - ref) * a.scale_log2), sum);
+                    }
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; ++c) {
+                        float v[32] = {};
+#pragma unroll 3
+                        for (int i = 0; i < n; ++i) {
+                            const float *pc = slot_of(from + i * step);
+                            const float g = fast_ex2((__ldcg(pc + 32 * D + lane) - ref) * a.scale_log2);
+                            float4 u[8];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) u[j] = __ldcg(reinterpret_cast<const float4 *>(pc) + (8 * c + j) * 32 + lane);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                v[4 * j] = fmaf(u[j].x, g, v[4 * j]);
+                                v[4 * j + 1] = fmaf(u[j].y, g, v[4 * j + 1]);
+                                v[4 * j + 2] = fmaf(u[j].z, g, v[4 * j + 2]);
+                                v[4 * j + 3] = fmaf(u[j].w, g, v[4 * j + 3]);
+                            }
+                        }
+                        sink(c, v);
                     }
                 };
-                tc_fence_after_sync();
-                bool write = first == final;
-                if (row0 >= rows) {  // none of the warp's rows is there
-                    write = false;
-                    if (shared) b_done();
-                } else if (write) {
-                    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+                // Many parts are joined in two steps, groups first, since one warp reads a part in more than a microsecond.  A
+                // CTA begins at most one shared item and continues at most one, so a counter per CTA, warp and use is enough.
+                int span = 1, n = parts;
+                bool go = true;
+                if (parts > kJoinAtOnce) {
+                    span = (int)ceilf(sqrtf((float)parts));
+                    n = (parts + span - 1) / span;
+                    const int group = ((int)blockIdx.x - first) / span, from = first + group * span;
+                    const int members = min(span, final - from + 1);
+                    go = last_of(a.tickets + (from * 3 + (group == 0 ? 1 : 2)) * 8 + warp, members);
+                    if (go) {  // the group's parts become one, in the place of its first
+                        float top, sum;
+                        float *to_slot = slot_of(from);
+                        join(from, 1, members, top, sum, [&](int c, float(&v)[32]) {
 #pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
-                        float o[32];
-                        load_o(c, o);
-                        auto g = [&](int i) { return o[i] * inv; };
+                            for (int j = 0; j < 8; ++j)
+                                *(reinterpret_cast<float4 *>(to_slot) + (8 * c + j) * 32 + lane) =
+                                    make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                        });
+                        to_slot[32 * D + lane] = top;
+                        to_slot[32 * D + 32 + lane] = sum;
+                    }
+                }
+                if (go && last_of(a.tickets + first * 3 * 8 + warp, n)) {
+                    // the last for these rows joins what there is, in the order of its keys
+                    write = true;
+                    float top, sum;
+                    join(first, span, n, top, sum, [&](int c, float(&v)[32]) {
+                        const float w = sum > 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             *reinterpret_cast<uint4 *>(chunk_at(lane, 4 * c + i)) =
-                                make_uint4(Half2Of<T>::pack(g(8 * i), g(8 * i + 1)), Half2Of<T>::pack(g(8 * i + 2), g(8 * i + 3)),
-                                           Half2Of<T>::pack(g(8 * i + 4), g(8 * i + 5)), Half2Of<T>::pack(g(8 * i + 6), g(8 * i + 7)));
-                    }
-                    if (shared) b_done();
-                } else {
-                    // [slot of the CTA][warp]: columns in vectors of four, 32 rows each
-                    const int parts = final - first + 1;
-                    auto slot_of = [&](int cta) {
-                        return a.partials + ((long long)(2 * cta + (cta == first ? 1 : 0)) * 8 + warp) * C::kWarpPartial;
-                    };
-                    float *part = slot_of((int)blockIdx.x);
-#pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
-                        float o[32];
-                        load_o(c, o);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            *reinterpret_cast<float4 *>(part + ((8 * c + i) * 32 + lane) * 4) =
-                                make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-                    }
-                    if (shared) b_done();
-                    part[32 * D + lane] = m;
-                    part[32 * D + 32 + lane] = l;
-                    // whether this warp is the last of n to arrive at a counter; then the others' parts can be read
-                    auto last_of = [&](int *ticket, int n) {
-                        __threadfence();
-                        __syncwarp();
-                        int before = 0;
-                        if (lane == 0) {
-                            before = atomicAdd(ticket, 1);
-                            if (before == n - 1) *ticket = 0;  // zero again for the next launch
-                        }
-                        before = __shfl_sync(0xffffffffu, before, 0);
-                        __threadfence();
-                        return before == n - 1;
-                    };
-                    // joins parts of the CTAs from, from + step, ...: maximum and sum, then 32 columns at a time to `sink`
-                    auto join = [&](int from, int step, int n, float &top, float &sum, auto &&sink) {
-                        top = -INFINITY;
-                        sum = 0.0f;
-                        for (int h = 0; h < n; h += 8) {  // eight loads on the way; behind the last part, it once more
-                            float m8[8];
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) m8[i] = __ldcg(slot_of(from + min(h + i, n - 1) * step) + 32 * D + lane);
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) top = fmaxf(top, m8[i]);
-                        }
-                        const float ref = top == -INFINITY ? 0.0f : top;
-                        for (int h = 0; h < n; h += 8) {
-                            float m8[8], l8[8];
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const float *pc = slot_of(from + min(h + i, n - 1) * step) + 32 * D + lane;
-                                m8[i] = __ldcg(pc);
-                                l8[i] = __ldcg(pc + 32);
-                            }
-#pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                if (h + i < n) sum = fmaf(l8[i], fast_ex2((m8[i] - ref) * a.scale_log2), sum);
-                        }
-#pragma unroll 1
-                        for (int c = 0; c < D / 32; ++c) {
-                            float v[32] = {};
-#pragma unroll 3
-                            for (int i = 0; i < n; ++i) {
-                                const float *pc = slot_of(from + i * step);
-                                const float g = fast_ex2((__ldcg(pc + 32 * D + lane) - ref) * a.scale_log2);
-                                float4 u[8];
-#pragma unroll
-                                for (int j = 0; j < 8; ++j) u[j] = __ldcg(reinterpret_cast<const float4 *>(pc) + (8 * c + j) * 32 + lane);
-#pragma unroll
-                                for (int j = 0; j < 8; ++j) {
-                                    v[4 * j] = fmaf(u[j].x, g, v[4 * j]);
-                                    v[4 * j + 1] = fmaf(u[j].y, g, v[4 * j + 1]);
-                                    v[4 * j + 2] = fmaf(u[j].z, g, v[4 * j + 2]);
-                                    v[4 * j + 3] = fmaf(u[j].w, g, v[4 * j + 3]);
-                                }
-                            }
-                            sink(c, v);
-                        }
-                    };
-                    // Many parts are joined in two steps, groups first, since one warp reads a part in more than a microsecond.  A
-                    // CTA begins at most one shared item and continues at most one, so a counter per CTA, warp and use is enough.
-                    int span = 1, n = parts;
-                    bool go = true;
-                    if (parts > kJoinAtOnce) {
-                        span = (int)ceilf(sqrtf((float)parts));
-                        n = (parts + span - 1) / span;
-                        const int group = ((int)blockIdx.x - first) / span, from = first + group * span;
-                        const int members = min(span, final - from + 1);
-                        go = last_of(a.tickets + (from * 3 + (group == 0 ? 1 : 2)) * 8 + warp, members);
-                        if (go) {  // the group's parts become one, in the place of its first
-                            float top, sum;
-                            float *to_slot = slot_of(from);
-                            join(from, 1, members, top, sum, [&](int c, float(&v)[32]) {
-#pragma unroll
-                                for (int j = 0; j < 8; ++j)
-                                    *(reinterpret_cast<float4 *>(to_slot) + (8 * c + j) * 32 + lane) =
-                                        make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-                            });
-                            to_slot[32 * D + lane] = top;
-                            to_slot[32 * D + 32 + lane] = sum;
-                        }
-                    }
-                    if (go && last_of(a.tickets + first * 3 * 8 + warp, n)) {
-                        // the last for these rows joins what there is, in the order of its keys
-                        write = true;
-                        float top, sum;
-                        join(first, span, n, top, sum, [&](int c, float(&v)[32]) {
-                            const float w = sum > 0.0f ? 1.0f / sum : 0.0f;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                *reinterpret_cast<uint4 *>(chunk_at(lane, 4 * c + i)) =
-                                    make_uint4(Half2Of<T>::pack(v[8 * i] * w, v[8 * i + 1] * w),
-                                               Half2Of<T>::pack(v[8 * i + 2] * w, v[8 * i + 3] * w),
-                                               Half2Of<T>::pack(v[8 * i + 4] * w, v[8 * i + 5] * w),
-                                               Half2Of<T>::pack(v[8 * i + 6] * w, v[8 * i + 7] * w));
-                        });
-                    }
+                                make_uint4(Half2Of<T>::pack(v[8 * i] * w, v[8 * i + 1] * w),
+                                           Half2Of<T>::pack(v[8 * i + 2] * w, v[8 * i + 3] * w),
+                                           Half2Of<T>::pack(v[8 * i + 4] * w, v[8 * i + 5] * w),
+                                           Half2Of<T>::pack(v[8 * i + 6] * w, v[8 * i + 7] * w));
+                    });
                 }
-                if (write) {
-                    __syncwarp();
-#pragma unroll
-                    for (int i = 0; i < kChunks; ++i) {
-                        const int row = i * kRowsPerPass + pass_row, r = row0 + row;
-                        const uint4 v = *reinterpret_cast<const uint4 *>(chunk_at(row, pass_chunk));
-                        if (r < rows) {
-                            const int tok = a.by_group.div(r), head = head0 + r - tok * a.group;
-                            *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + (q0 + tok) * a.o_ts + head * a.o_hs +
-                                                       pass_chunk * 8) = v;
-                        }
-                    }
-                    __syncwarp();
-                }
-                tc_fence_before_sync();  // O has been read before the next run's first product, which waits for p_ready
             }
+            if (write) {
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < kChunks; ++i) {
+                    const int row = i * kRowsPerPass + pass_row, r = row0 + row;
+                    const uint4 v = *reinterpret_cast<const uint4 *>(chunk_at(row, pass_chunk));
+                    if (r < rows) {
+                        const int tok = a.by_group.div(r), head = head0 + r - tok * a.group;
+                        *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + (q0 + tok) * a.o_ts + head * a.o_hs +
+                                                   pass_chunk * 8) = v;
+                    }
+                }
+                __syncwarp();
+            }
+            tc_fence_before_sync();  // O has been read before the next run's first product, which waits for p_ready
             if (more) load_q(it.rt * kChunkRows + tile * 128 + sub * 32);
         }
     }
