@@ -342,8 +342,9 @@ typedef struct {
  * are never read.  Rows behind q_starts[n_seqs] belong to no sequence and are left as they are.
  * The arrays are read by the kernels, never by the host, so a captured graph follows what they hold at replay.
  * max_new_tokens is the caller's bound on the new tokens of one sequence; it chooses the kernel and nothing else: a
- * wrong bound costs time, not results.
- * A new token whose position is negative (kv_lens[s] smaller than its new tokens) is not appended, and attends to nothing.
+ * wrong bound costs time, not results (64 sequences of one token taken for 64 tokens of one: 1.3 to 1.8 times the time).
+ * A new token whose position is negative (kv_lens[s] smaller than its new tokens) is not appended, its row of q_out is left
+ * as it was, and it attends to nothing.
  * A length beyond max_pages * page_tokens, or a page outside [0, n_pages) where a key is needed, is not accessed: the
  * call's results for that sequence are undefined, and the next entry point returns 1 once, as for a wait that ran out. */
 typedef struct {
@@ -392,12 +393,17 @@ int b200_w8a8_kv_append(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batc
  *   causal_block = 0:     every key of its sequence;
  *   causal_block = F > 0: keys up to the end of p's block of F positions, j < (p / F + 1) * F (1: plain causal; the tokens
  *                         of a frame: every frame sees itself and what came before);
- *   window = W > 0 (needs causal_block): of those, j >= (p / F + 1) * F - W, the last W up to the end of the block.
+ *   window = W > 0 (needs causal_block): of those, j >= (p / F + 1) * F - W, the last W up to the end of the block.  All tokens
+ *                         of a block see the same keys, so a window counts in whole frames: W = F sees the own frame, W = 2 F
+ *                         the one before it too.  W < F hides the beginning of the own block, the token itself where it stands
+ *                         there; and where the sequence ends inside a block, fewer than W of the keys are there, none if it
+ *                         ends before the window begins.
  * A token that sees no key, or all of whose scores are minus infinity, gets zeros; a NaN or a plus infinity among the scores
  * makes its output NaN.  Keys and values behind a sequence's length may hold anything; a value that stands within
  * the length and is hidden from a token counts with weight zero, so a NaN or infinity there spreads as zero times it.
  * q and out have the cache's type, strides in elements (multiples of 8) and 16-byte aligned pointers; they may not overlap.
- * Scores, softmax and sums are fp32; weights are rounded to the cache's type for the product with the values.
+ * Scores, softmax and sums are fp32; weights are rounded to the cache's type for the product with the values, fp16 ones with a
+ * factor that cancels, so that small ones are kept.
  * scale must be positive and finite, n_heads a multiple of the cache's n_kv_heads.
  * workspace: at least b200_w8a8_paged_attention_workspace_size bytes on the current device, 256-byte aligned, its first
  * 32768 bytes zero before the first call; every call leaves them zero, except one whose wait ran out: zero them again
@@ -487,8 +493,9 @@ typedef struct {
  * (src/world_cuda.cu:1819-1882 and 2058-2330) with each quantize -> int8 GEMM -> dequant triple
  * fused into one GEMM launch -- 13 launches per layer instead of 16 and no T x hidden int32 scratch.
  * The context owns activation scratch for up to max_tokens rows (device_bytes reports it); weights are
- * read in `w_layout` where the caller keeps them.  d_head must be 64 (see b200_w8a8_linear_qkv_heads)
- * and n_heads * d_head == d_model.  rope_cos / rope_sin come from b200_w8a8_rope_tables, once per frame.
+ * read in `w_layout` where the caller keeps them.  d_head must be 64 (see b200_w8a8_linear_qkv_heads; for
+ * b200_w8a8_layer_forward_paged below, 64 or 128) and n_heads * d_head == d_model.  rope_cos / rope_sin come from
+ * b200_w8a8_rope_tables, once per frame.
  * tokens_next may be the same buffer as tokens. */
 void *b200_w8a8_layer_ctx_create(int max_tokens, int d_model, int n_heads, int n_kv_heads, int d_head, int d_hidden,
                                  float eps, int w_layout);

@@ -510,7 +510,9 @@ class PagedKVCache:
 class PagedBatch:
     """The sequences of a call (see b200_w8a8_kv_batch): int32 CUDA tensors page_table [seqs, pages], q_starts [seqs + 1]
     and kv_lens [seqs], which the kernels read at run time, so they may be updated in place between calls.
-    max_new_tokens: the caller's bound on the new tokens of one sequence (None: the rows of the call)."""
+    max_new_tokens: the caller's bound on the new tokens of one sequence (None: the rows of the call).  It chooses between a
+    kernel for few rows and one for many; give it when decoding a batch, where None takes the second: 64 sequences of one
+    token over up to 8191 keys 334 us instead of 246, over up to 1000 keys 77 instead of 44."""
 
     def __init__(self, page_table, q_starts, kv_lens, max_new_tokens=None):
         import torch
@@ -617,7 +619,8 @@ def make_attention_workspace(cache):
 
 def paged_attention(q, cache, batch, scale=None, causal_block=1, window=0, out=None, workspace=None):
     """Attention of the new tokens' queries q [tokens, heads, d_head] (the cache's type) over the cache; returns out, like q.
-    causal_block 0: every key; 1: causal; F: causal by blocks of F positions.  window: keys seen, 0 for all.
+    causal_block 0: every key; 1: causal; F: causal by blocks of F positions.  window: keys seen up to the end of the block, 0 for
+    all; one smaller than causal_block hides the beginning of a token's own block from it.
     scale: 1 / sqrt(d_head) when None.  workspace: from make_attention_workspace (a fresh one when None)."""
     import torch
     d, index = cache.d_head, cache.index

@@ -10,9 +10,10 @@
 // token to itself; with few, two, four or the eight warps of a CTA share one.  Each warp finds its token's place by itself, while
 // its first heads are on the way: 32 probes at a time into the sequences' starts, then length and page; no barrier.
 //
-// Measured: 98348 fp16 rows (32 + 2 x 16 heads of 64) 287 to 295 us = 5.6 TB/s, 86 % of a plain copy (issue slots 62 % busy); a
+// Measured: 98348 fp16 rows (32 + 2 x 16 heads of 64) 287 to 295 us = 5.6 TB/s, 86 % of a plain copy (issue slots 68 % busy); a
 // frame of 512 fp32 rows 3.8 us, 128 bf16 rows of 128 sequences 4.9 us, one row 2.6 us.  With the places looked up by the CTA
 // behind barriers, and addresses and arithmetic element by element, the first took 327 us; without several heads in flight 401.
+// Four CTAs per SM leave 64 registers a thread, over which the rotation of halves from 16-bit rows spills 4 to 12 bytes.
 #include "paged_kv.cuh"
 
 namespace b200 {
@@ -267,7 +268,8 @@ int kv_append(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *batch, 
     p.norm = x->norm != 0; p.eps = x->eps; p.q_weight = x->q_weight; p.k_weight = x->k_weight;
     p.cos = x->rope_cos; p.sin = x->rope_sin; p.by_position = x->rope_by_position != 0; p.rope_rows = x->rope_rows;
     // 148 SMs hold 4736 of these warps.  Few rows are spread over them, many are better off with a place looked up once and all
-    // heads of a row behind it.  Measured with 8 / 4 / 2 / 1 warps a row (64 heads of 64, fp16; 48 heads of 128, bf16), us:
+    // heads of a row behind it.  The number of heads does not enter: of few, most of a row's warps have none.  Measured with
+    // 8 / 4 / 2 / 1 warps a row (64 heads of 64, fp16; 48 heads of 128, bf16), us:
     //      400 rows   3.9 /  4.6 /  5.6 /  8.0
     //      800 rows   5.8 /  5.0 /  7.4 /  9.0      8.7 /  8.4 / 12.0 / 15.0
     //     1600 rows   8.8 /  7.4 /  7.9 / 12.6     13.6 / 13.0 / 13.3 / 21.1

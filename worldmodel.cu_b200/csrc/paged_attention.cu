@@ -10,8 +10,8 @@
 // weights are rounded once each to the cache's type; scores, maxima, sums and O are fp32.
 //
 // Measured: 64 sequences of up to 8191 keys (32 / 8 heads of 128, bf16) 246 us = 6.5 TB/s, what a plain copy reaches; one of
-// 131071 keys 94 us = 5.7 TB/s (of the rest about 5 us are launch, plan and first loads, 4 us the join); one of 777 keys
-// (32 / 16 heads of 64) 9.6 us, all latency: plan, first loads, parts and join, each behind the one before.
+// 131071 keys 95 us = 5.7 TB/s (of the rest about 5 us are launch, plan and first loads, 4 us the join); one of 777 keys
+// (32 / 16 heads of 64) 10 us, all latency: plan, first loads, parts and join, each behind the one before.
 #include <algorithm>
 #include <mutex>
 
@@ -459,6 +459,8 @@ int paged_attention(const b200_w8a8_kv_cache *cache, const b200_w8a8_kv_batch *b
     const bool bf = cache->dtype == B200_DT_BF16;
     // One row tile of 16 rows: the rows kernel, bound by HBM whatever the group.  More rows would read every key again for each
     // row tile: measured with 20, 32 and 48 rows, the chunk kernel / the rows kernel, 49.7 / 52.0, 35.1 / 42.5 and 84 / 160 us.
+    // What a bound above the real numbers costs: 64 sequences x 1 token, 4 heads a key head, with a bound of 64 / of 1, 334 / 246 us
+    // over up to 8191 keys of 128, 77 / 44 us over up to 1000.
     const bool few = (long long)batch->max_new_tokens * a.group <= kRowTile;
     a.min_tiles = 2;  // measured 2 / 4 / 8 / 16 units at least: one sequence of 777 keys 9.7 / 11.2 / 13.8 / 18.9 us
     if (!few || !work_fits(cache, batch, a.group, kRowTile, kRowsKeyTile, kRowsExtra))

@@ -13,10 +13,11 @@
 // transposed.  Rows of V outside the sequence are zeroed in shared memory before their product, since 0 x NaN is no zero.
 // An item of at most 128 rows has no second row tile: both accumulators work on it, KV tiles in turn.
 //
-// Measured: a prompt of 8192 tokens (32 / 8 heads of 128, bf16, causal) 470 us = 1.17 PFLOP/s, 71 % of the rate of a large
-// library product; a frame of 512 tokens over 8704 keys (32 / 16 heads of 64, fp16) 62.5 us,
-// 80 rows of 16 sequences of up to 4001 keys (32 / 2 heads of 128) 27.9 us.  The tensor pipe is busy 56 % of the
-// cycles, the special-function unit 43 %, the issue slots 43 %: what bounds the loop is the chain scores -> maximum -> weights
+// Measured in a graph of a few passes: a prompt of 8192 tokens (32 / 8 heads of 128, bf16, causal) 475 us = 1.16 PFLOP/s, 70 % of
+// the rate of a large library product; repeated without a pause it runs into the power cap, 545 us = 1.01 PFLOP/s.  A frame
+// of 512 tokens over 8704 keys (32 / 16 heads of 64, fp16) 65 to 68 us, 80 rows of 16 sequences of up to 4001 keys (32 / 2 heads of
+// 128) 28 us.  In the prompt the tensor pipe is busy 60 % of the
+// cycles, the special-function unit 45 %, the issue slots 46 %: what bounds the loop is the chain scores -> maximum -> weights
 // -> product of a row tile (about 3400 cycles a KV tile, of which the products are 1000), of which two run against each other.
 // Tried and slower: half a row per thread with sixteen softmax warps (563 us), KV tiles in halves with two score buffers (517),
 // a thread per row tile to issue products (583 when their batches mix, 501 when the softmax warps take turns), all
